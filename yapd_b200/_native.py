@@ -1,6 +1,7 @@
-"""ctypes binding of ``include/yapd_select.h`` (the library's C ABI).
+"""ctypes binding of ``include/yapd_select.h`` and ``include/yapd_cache.h`` (the
+library's C ABI).
 
-The structures below mirror the header field by field.  Loading fails loudly
+The structures below mirror the headers field by field.  Loading fails loudly
 when the in-tree library is missing: there is no CPU fallback.
 """
 from __future__ import annotations
@@ -33,6 +34,23 @@ EXPORTED = [
     "yapd_lmhead_workspace_size", "yapd_lmhead_select_step",
 ]
 YAPD_NOALLOC_MAX_POSITIONS = 16384
+
+# yapd_cache.h
+YAPD_CACHE_ABI_VERSION = 1
+YAPD_DTYPE_F16 = 2
+YAPD_STATUS_OUT_OF_PAGES = 16
+YAPD_STATUS_BAD_PAGE = 32
+YAPD_STATUS_SHARED_PAGE = 64
+YAPD_STATUS_BAD_SLOT = 128
+YAPD_STATUS_BAD_LENGTH = 256
+YAPD_MAX_NEW_TOKENS = 32
+YAPD_LOGPROBS_MAX_V = 1048576
+YAPD_LOGPROBS_MAX_TOP = 32
+CACHE_EXPORTED = [
+    "yapd_cache_abi_version", "yapd_cache_workspace_size", "yapd_attend",
+    "yapd_pages_reserve", "yapd_pages_fork", "yapd_pages_truncate", "yapd_pages_trim",
+    "yapd_pages_compact", "yapd_pages_copy", "yapd_token_logprobs",
+]
 
 
 class Sampling(C.Structure):
@@ -105,6 +123,48 @@ class LmheadArgs(C.Structure):
     ]
 
 
+class Cache(C.Structure):
+    _fields_ = [
+        ("layers", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("dtype", C.c_int32), ("slots", C.c_int32), ("max_pages", C.c_int32),
+        ("kv", C.c_void_p), ("stride_layer", C.c_int64), ("stride_page", C.c_int64),
+        ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("refs", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class AttendArgs(C.Structure):
+    _fields_ = [
+        ("cache", Cache),
+        ("layer", C.c_int32), ("B", C.c_int32), ("new_tokens", C.c_int32), ("heads", C.c_int32),
+        ("slots", C.c_void_p),
+        ("q", C.c_void_p), ("q_stride_req", C.c_int64), ("q_stride_pos", C.c_int64), ("q_stride_head", C.c_int64),
+        ("k", C.c_void_p), ("k_stride_req", C.c_int64), ("k_stride_pos", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v", C.c_void_p), ("v_stride_req", C.c_int64), ("v_stride_pos", C.c_int64), ("v_stride_head", C.c_int64),
+        ("out", C.c_void_p), ("out_stride_req", C.c_int64), ("out_stride_pos", C.c_int64),
+        ("out_stride_head", C.c_int64),
+        ("lse", C.c_void_p), ("scale", C.c_float), ("causal", C.c_int32),
+        ("window", C.c_int64), ("sinks", C.c_int64),
+    ]
+
+
+class PagesArgs(C.Structure):
+    _fields_ = [
+        ("cache", Cache),
+        ("n", C.c_int32), ("slots", C.c_void_p), ("src", C.c_void_p), ("dst", C.c_void_p),
+        ("tokens", C.c_int64), ("tokens_each", C.c_void_p), ("window", C.c_int64), ("sinks", C.c_int64),
+        ("granted", C.c_void_p), ("live", C.c_void_p),
+    ]
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [
+        ("R", C.c_int32), ("V", C.c_int32), ("top_n", C.c_int32), ("logits_dtype", C.c_int32),
+        ("logits", C.c_void_p), ("stride_row", C.c_int64), ("targets", C.c_void_p),
+        ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_logprobs", C.c_void_p), ("top_ids", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -139,7 +199,18 @@ def lib():
     h.yapd_lmhead_workspace_size.argtypes = [C.c_int32, C.c_int32]
     h.yapd_lmhead_select_step.restype = C.c_int
     h.yapd_lmhead_select_step.argtypes = [C.POINTER(LmheadArgs), C.c_void_p]
-    if h.yapd_abi_version() != YAPD_ABI_VERSION:
+    h.yapd_cache_abi_version.restype = C.c_int
+    h.yapd_cache_workspace_size.restype = C.c_size_t
+    h.yapd_cache_workspace_size.argtypes = [C.POINTER(Cache)]
+    h.yapd_attend.restype = C.c_int
+    h.yapd_attend.argtypes = [C.POINTER(AttendArgs), C.c_void_p]
+    for name in ("reserve", "fork", "truncate", "trim", "compact", "copy"):
+        f = getattr(h, "yapd_pages_" + name)
+        f.restype = C.c_int
+        f.argtypes = [C.POINTER(PagesArgs), C.c_void_p]
+    h.yapd_token_logprobs.restype = C.c_int
+    h.yapd_token_logprobs.argtypes = [C.POINTER(LogprobsArgs), C.c_void_p]
+    if h.yapd_abi_version() != YAPD_ABI_VERSION or h.yapd_cache_abi_version() != YAPD_CACHE_ABI_VERSION:
         raise RuntimeError("yapd_select ABI version mismatch")
     _lib = h
     return h

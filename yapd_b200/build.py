@@ -18,8 +18,9 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(LIBDIR, "libyapd_select.so")
-SOURCES = ["select_step.cu"]
-HEADERS = ["philox.cuh", "select_common.cuh", "lmhead_select.cuh"]
+SOURCES = ["select_step.cu", "paged_attend.cu", "paged_pages.cu", "token_logprobs.cu"]
+HEADERS = ["philox.cuh", "select_common.cuh", "lmhead_select.cuh", "serve_common.cuh"]
+ABI_HEADERS = ["yapd_select.h", "yapd_cache.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -42,7 +43,7 @@ def _stale() -> bool:
         return True
     t = os.path.getmtime(LIB)
     deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(ROOT, "include", "yapd_select.h"))
+    deps += [os.path.join(ROOT, "include", f) for f in ABI_HEADERS]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
@@ -52,7 +53,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
     tmp = LIB + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-o", tmp,
+    cmd = [nvcc_path(), *NVCC_FLAGS, "--threads", "0", "-I", os.path.join(ROOT, "include"), "-o", tmp,
            *[os.path.join(CSRC, f) for f in SOURCES]]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

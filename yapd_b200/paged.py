@@ -1,0 +1,301 @@
+"""A paged key-value cache and the attention that reads it.
+
+``PagedCache`` holds a pool of pages and the requests' tables into it, all on
+the device: the layout of a page is the reference's FlashInfer engine's
+(m8than/yapd ``chatterbox_flash/engines/flashinfer.py:110-115``, blocks of
+``(2, page_size, kv_heads, head_dim)``), the slots are the engines' request rows
+(``server/engine.py:332``).  One tick of an autoregressive engine
+(``server/engine_ar.py:382-422``) is::
+
+    cache.reserve(1)                            # room for the token of every slot
+    for layer in range(layers):
+        q, k, v = project(layer, hidden)        # (B, heads, D), (B, kv_heads, D) twice
+        hidden = finish(layer, cache.attend(layer, q, k, v))
+    token = sample_rows(head(hidden))
+
+A block-diffusion engine reserves its 16 positions once and calls ``attend``
+with ``causal=False`` at every step (``server/engine.py:512-515``): the block's
+keys and values are stored again each time and every position sees the block.
+
+Everything runs the kernels of ``libyapd_select.so`` on the current CUDA stream
+and synchronises nothing.  Lists of slots, pages and token counts are device
+tensors; what only the device can see wrong in them (a full pool, a slot listed
+twice) leaves the slot alone and sets bits of ``cache.status()``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.float32: N.YAPD_DTYPE_F32, torch.bfloat16: N.YAPD_DTYPE_BF16, torch.float16: N.YAPD_DTYPE_F16}
+
+
+def _rows(t: torch.Tensor, vec: int) -> torch.Tensor:
+    """``t`` itself if the kernels can read its rows of the last dimension, else a contiguous copy."""
+    st = t.stride()
+    if st[-1] != 1 or t.data_ptr() % 16 or any(s % vec for s in st[:-1]):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+class PagedCache:
+    """Pages ``kv`` ``(layers, pages, 2, page_size, kv_heads, head_dim)`` in
+    float32, bfloat16 or float16, with the tables of ``slots`` requests.
+
+    ``page_table`` ``(slots, max_pages)`` int32 (-1: no page), ``kv_len``
+    ``(slots,)`` int64 and ``refs`` ``(pages,)`` int32 are the caller's tensors,
+    updated in place; ``PagedCache.empty`` makes them.  Each page's block has to
+    be contiguous; the first two strides of ``kv`` are free.  ``head_dim`` is 32,
+    64, 96 or 128.  The cache's calls share a workspace: they are ordered on one
+    stream, or by events where a program uses several.
+    """
+
+    def __init__(self, kv: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, refs: torch.Tensor):
+        if not kv.is_cuda:
+            raise ValueError("PagedCache runs on CUDA tensors only (no CPU fallback)")
+        if kv.dtype not in _DTYPES:
+            raise TypeError(f"kv must be float32, bfloat16 or float16, got {kv.dtype}")
+        if kv.dim() != 6 or kv.shape[2] != 2:
+            raise ValueError("kv must be (layers, pages, 2, page_size, kv_heads, head_dim)")
+        if kv.shape[5] not in (32, 64, 96, 128):
+            raise ValueError(f"head_dim must be 32, 64, 96 or 128, got {kv.shape[5]}")
+        if kv.numel() == 0 or not kv[0, 0].is_contiguous():
+            raise ValueError("each page of kv must be contiguous, and there must be one")
+        layers, pages = kv.shape[:2]
+        dev = kv.device
+        slots = kv_len.shape[0] if kv_len.dim() == 1 else 0
+        if slots < 1 or page_table.dim() != 2 or page_table.shape[0] != slots:
+            raise ValueError("kv_len must be (slots,) and page_table (slots, max_pages)")
+        for name, t, dtype, shape in (("page_table", page_table, torch.int32, tuple(page_table.shape)),
+                                      ("kv_len", kv_len, torch.int64, (slots,)), ("refs", refs, torch.int32, (pages,))):
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{name} must be a contiguous {dtype} {shape} tensor on {dev}")
+        self.kv, self.page_table, self.kv_len, self.refs = kv, page_table, kv_len, refs
+        self.slots, self.device = slots, dev
+        self._vec = 16 // kv.element_size()
+        self._heads, self._dim = kv.shape[4], kv.shape[5]
+        c = N.Cache()
+        c.layers, c.pages, _, c.page_size, c.kv_heads, c.head_dim = kv.shape
+        c.dtype, c.slots, c.max_pages = _DTYPES[kv.dtype], slots, page_table.shape[1]
+        c.kv = kv.data_ptr()
+        c.stride_layer, c.stride_page = kv.stride(0), kv.stride(1)
+        c.page_table, c.kv_len, c.refs = page_table.data_ptr(), kv_len.data_ptr(), refs.data_ptr()
+        self._lib = N.lib()
+        need = self._lib.yapd_cache_workspace_size(C.byref(c))
+        if need == 0:
+            raise ValueError("page_size, kv_heads or max_pages * page_size is out of range")
+        self._workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
+        c.workspace, c.workspace_bytes = self._workspace.data_ptr(), need
+        self._attend, self._pages = N.AttendArgs(), N.PagesArgs()
+        self._attend.cache = self._pages.cache = c
+
+    @classmethod
+    def empty(cls, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int,
+              max_pages: int, dtype=torch.bfloat16, device="cuda") -> "PagedCache":
+        """A pool of free pages and empty slots, each with room for ``max_pages`` pages."""
+        dev = torch.device(device)
+        if dev.type == "cuda" and dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        return cls(torch.empty(layers, pages, 2, page_size, kv_heads, head_dim, dtype=dtype, device=dev),
+                   torch.full((slots, max_pages), -1, dtype=torch.int32, device=dev),
+                   torch.zeros(slots, dtype=torch.int64, device=dev),
+                   torch.zeros(pages, dtype=torch.int32, device=dev))
+
+    # ------------------------------------------------------------- attention
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None, *,
+               slots: torch.Tensor | None = None, causal: bool = True, window: int = 0, sinks: int = 0,
+               scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+        """Attention of each request's last tokens over its pages in ``layer``.
+
+        ``q`` is ``(B, heads, D)`` for one new token per request or ``(B, T,
+        heads, D)`` for its last ``T <= 32``, with ``heads`` a multiple of
+        ``kv_heads``; row ``b`` is slot ``slots[b]`` (int32), or slot ``b``.
+        ``k`` and ``v`` (``q``'s shape with ``kv_heads``) are stored in the
+        tokens' pages by the same call; without them the pages are only read.
+        The tokens are part of ``kv_len`` already (``reserve``).
+
+        Query ``i``, at position ``p = kv_len - T + i``, sees the tokens of its
+        request, up to ``p`` if ``causal``, and with ``window > 0`` only those
+        after ``p - window`` and the first ``sinks``.  ``scale`` is ``D ** -0.5``
+        if not given.  A query that sees nothing gets zeros (and an ``lse`` of
+        -inf).  Returns the output in ``q``'s shape and type, with
+        ``return_lse`` also the ``(B, T, heads)`` or ``(B, heads)`` float32
+        logarithms of the softmax's sums.
+        """
+        a, kv = self._attend, self.kv
+        shape = q.shape
+        if q.dim() == 3:
+            q = q.unsqueeze(1)
+            k = k if k is None or k.dim() != 3 else k.unsqueeze(1)
+            v = v if v is None or v.dim() != 3 else v.unsqueeze(1)
+        if q.dim() != 4 or q.shape[3] != self._dim or q.shape[2] % self._heads or q.shape[2] == 0:
+            raise ValueError(f"q must be (B, [T,] heads, {self._dim}) with heads a multiple of {self._heads}, "
+                             f"got {tuple(shape)}")
+        B, T, H, D = q.shape
+        if not 1 <= T <= N.YAPD_MAX_NEW_TOKENS:
+            raise ValueError(f"1 to {N.YAPD_MAX_NEW_TOKENS} new tokens, got {T}")
+        if q.dtype != kv.dtype or q.device != kv.device:
+            raise TypeError(f"q must be {kv.dtype} on {kv.device}")
+        if not 0 <= layer < kv.shape[0]:
+            raise ValueError(f"layer {layer} of {kv.shape[0]}")
+        if sinks < 0:
+            raise ValueError("sinks must not be negative")
+        if slots is not None:
+            self._check_list("slots", slots, B)
+        elif B > self.slots:
+            raise ValueError(f"{B} requests, but {self.slots} slots")
+        q = _rows(q, self._vec)
+        a.layer, a.B, a.new_tokens, a.heads = layer, B, T, H
+        a.slots = None if slots is None else slots.data_ptr()
+        a.q = q.data_ptr()
+        a.q_stride_req, a.q_stride_pos, a.q_stride_head, _ = q.stride()
+        if k is None and v is None:
+            a.k = a.v = None
+        else:
+            if k is None or v is None:
+                raise ValueError("k and v come together")
+            want = (B, T, self._heads, D)
+            if k.shape != want or v.shape != want:
+                raise ValueError(f"k and v must be {want}, got {tuple(k.shape)} and {tuple(v.shape)}")
+            if k.dtype != kv.dtype or v.dtype != kv.dtype or k.device != kv.device or v.device != kv.device:
+                raise TypeError(f"k and v must be {kv.dtype} on {kv.device}")
+            k, v = _rows(k, self._vec), _rows(v, self._vec)
+            a.k, a.v = k.data_ptr(), v.data_ptr()
+            a.k_stride_req, a.k_stride_pos, a.k_stride_head, _ = k.stride()
+            a.v_stride_req, a.v_stride_pos, a.v_stride_head, _ = v.stride()
+        if out is None:
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        elif out.shape != shape or out.dtype != q.dtype or out.device != q.device or \
+                _rows(out, self._vec) is not out:
+            raise ValueError(f"out must be a {tuple(shape)} {q.dtype} tensor on {q.device} whose rows are aligned")
+        o = out.unsqueeze(1) if out.dim() == 3 else out
+        a.out = out.data_ptr()
+        a.out_stride_req, a.out_stride_pos, a.out_stride_head, _ = o.stride()
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        a.lse = lse.data_ptr() if return_lse else None
+        a.scale = D ** -0.5 if scale is None else scale
+        a.causal, a.window, a.sinks = 1 if causal else 0, window, sinks
+        self._call(self._lib.yapd_attend, a)
+        return (out, lse) if return_lse else out
+
+    # ----------------------------------------------------------------- pages
+
+    def reserve(self, tokens, slots: torch.Tensor | None = None) -> torch.Tensor:
+        """Room for ``tokens`` more (an int, or int64 ``(n,)``) in each slot of
+        the list, in its order; ``kv_len`` grows.  A partly filled last page that
+        other slots hold too is copied first.  Returns ``(n,)`` bool: the first
+        slot that the pool has no room for, and all after it, are refused."""
+        if isinstance(tokens, int) and tokens < 0:
+            raise ValueError("tokens must not be negative")
+        p = self._listed(slots)
+        self._tokens(tokens, p.n)
+        granted = torch.empty(p.n, dtype=torch.bool, device=self.device)
+        p.granted = granted.data_ptr()
+        self._call(self._lib.yapd_pages_reserve, p)
+        return granted
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """The empty slots ``dst`` become copies of ``src`` and share their pages
+        (both int32 ``(n,)``; no slot is in both)."""
+        p = self._listed(dst)
+        self._check_list("src", src, p.n)
+        p.src = src.data_ptr()
+        self._call(self._lib.yapd_pages_fork, p)
+
+    def truncate(self, tokens, slots: torch.Tensor | None = None) -> None:
+        """Takes the last ``tokens`` (an int, or int64 ``(n,)``) from each slot."""
+        if isinstance(tokens, int) and tokens < 0:
+            raise ValueError("tokens must not be negative")
+        p = self._listed(slots)
+        self._tokens(tokens, p.n)
+        self._call(self._lib.yapd_pages_truncate, p)
+
+    def free(self, slots: torch.Tensor | None = None) -> None:
+        """Empties the slots; pages that no other slot holds become free."""
+        p = self._listed(slots)
+        p.tokens, p.tokens_each = -1, None
+        self._call(self._lib.yapd_pages_truncate, p)
+
+    def trim(self, window: int, sinks: int = 0, slots: torch.Tensor | None = None) -> None:
+        """Gives up the pages that attention with this ``window`` and ``sinks``
+        no longer sees, from the slots' next token on."""
+        if window < 1 or sinks < 0:
+            raise ValueError("window must be positive and sinks not negative")
+        p = self._listed(slots)
+        p.window, p.sinks = window, sinks
+        self._call(self._lib.yapd_pages_trim, p)
+
+    def compact(self) -> torch.Tensor:
+        """Moves the live pages to the pool's lowest numbers, in all layers and
+        tables.  Returns their number, a ``(1,)`` int32 device tensor."""
+        p = self._listed(None)
+        live = torch.empty(1, dtype=torch.int32, device=self.device)
+        p.live = live.data_ptr()
+        self._call(self._lib.yapd_pages_compact, p)
+        return live
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Copies pages ``src`` to ``dst`` (int32 ``(n,)``) in all layers; no page
+        is both read and written, or written twice."""
+        p = self._pages
+        if dst.dim() != 1 or dst.shape[0] > self.kv.shape[1]:
+            raise ValueError("dst must be (n,) with n at most the number of pages")
+        self._check_list("dst", dst, dst.shape[0])
+        self._check_list("src", src, dst.shape[0])
+        p.n, p.src, p.dst = dst.shape[0], src.data_ptr(), dst.data_ptr()
+        self._call(self._lib.yapd_pages_copy, p)
+
+    # ---------------------------------------------------------------- status
+
+    def status(self) -> int:
+        """The status word (``YAPD_STATUS_*`` bits; synchronises the stream)."""
+        word = C.c_uint32(0)
+        N.check(self._lib.yapd_read_status(C.c_void_p(self._workspace.data_ptr()), self._stream(), C.byref(word)))
+        return word.value
+
+    def clear_status(self) -> None:
+        N.check(self._lib.yapd_clear_status(C.c_void_p(self._workspace.data_ptr()), self._stream()))
+
+    # --------------------------------------------------------------- private
+
+    def _stream(self) -> C.c_void_p:
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _call(self, entry, args) -> None:
+        if torch.cuda.current_device() == self.device.index:
+            rc = entry(args, self._stream())
+        else:
+            with torch.cuda.device(self.device):
+                rc = entry(args, self._stream())
+        if rc:
+            N.check(rc)
+
+    def _check_list(self, name: str, t: torch.Tensor, n: int) -> None:
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != self.device or \
+                (n > 1 and t.stride(0) != 1):
+            raise ValueError(f"{name} must be a contiguous int32 ({n},) tensor on {self.device}")
+
+    def _listed(self, slots: torch.Tensor | None):
+        p = self._pages
+        if slots is None:
+            p.n, p.slots = self.slots, None
+        else:
+            if slots.dim() != 1 or slots.shape[0] > self.slots:
+                raise ValueError(f"slots must be (n,) with n <= {self.slots}")
+            self._check_list("slots", slots, slots.shape[0])
+            p.n, p.slots = slots.shape[0], slots.data_ptr()
+        return p
+
+    def _tokens(self, tokens, n: int) -> None:
+        p = self._pages
+        if isinstance(tokens, torch.Tensor):
+            if tokens.dtype != torch.int64 or tuple(tokens.shape) != (n,) or tokens.device != self.device or \
+                    not tokens.is_contiguous():
+                raise ValueError(f"tokens must be an int or a contiguous int64 ({n},) tensor on {self.device}")
+            p.tokens, p.tokens_each = 0, tokens.data_ptr()
+        else:
+            p.tokens, p.tokens_each = int(tokens), None
