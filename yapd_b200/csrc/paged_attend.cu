@@ -13,6 +13,7 @@
 // workspace, and the CTA that arrives last joins them in their order.  No CTA
 // waits for another one.
 #include <atomic>
+#include <cmath>
 
 #include "serve_common.cuh"
 
@@ -29,20 +30,22 @@ struct Attend {
   Div groups;        // query heads per key head
   int group;
   int rows;          // new_tokens * group: query rows that share a key head
-  int wr;            // warps along the rows: 1, 2, 4
+  int wr;            // warps along the rows: 1, 2, 4 (1 unless M = 16)
   int hg;            // key heads of a unit: 1, 2, 4
   int head_groups, row_blocks;
-  float scale_log2;
+  uint32_t negate;   // sign bits of the queries to turn
+  float scale_log2;  // not negative
   int* counters;     // (gridDim): arrivals at a cut piece that starts in the CTA
   float* partials;   // (gridDim, 2, kMaxRows, D + 2)
 };
 
 // ------------------------------------------------------------ shapes by type
 
-template <class T, int D>
+// M: query rows of a warp, 4, 8 or 16.
+template <class T, int D, int M>
 struct Shape {
   // rows of keys in a stage, and as many of values
-  static constexpr int kRows = sizeof(T) == 2 ? (D <= 64 ? 128 : 64) : (D == 32 ? 64 : 32);
+  static constexpr int kRows = sizeof(T) == 2 ? (D == 32 ? 128 : 64) : (D == 32 ? 64 : 32);
   static constexpr int kStep = kRows / kWarps < 32 ? kRows / kWarps : 32;  // keys of one softmax step
   static constexpr int kPitch = D * sizeof(T) + 16;  // bytes: eight rows' 16-byte chunks fall in different banks
   static constexpr int kHalf = kRows * kPitch;
@@ -51,11 +54,14 @@ struct Shape {
   static constexpr int kChunks = D * sizeof(T) / 16;
   static constexpr int kLoads = kRows * kChunks / kThreads;
   static constexpr int kJoinPitch = D + 4;           // floats
-  static constexpr int kQ = sizeof(T) == 4 ? kWarps * 16 * (D + 4) * 4 : 0;
-  static constexpr int kMaxKeys = kRows;             // keys of a tile: kRows / hg
-  static constexpr int kSmem = kStages * kStage + kQ + (kStages + 1) * kMaxKeys * 8 + 2 * kWarps * 16 * 4;
-  static_assert(kWarps * 16 * kJoinPitch * 4 <= kStage, "the join fits a stage");
-  static_assert(kRows * kChunks % kThreads == 0, "");
+  static constexpr int kWords = kRows / 32;          // of a mask of keys
+  static constexpr int kQuery = sizeof(T) == 4 ? M * (D + 4) : 0;  // floats of a warp's queries in shared memory
+  static constexpr int kSmem = kStages * kStage + kWarps * kQuery * 4 + 2 * kRows * 8;
+  // CTAs of an SM: as many as its 228 KB hold, and no more than leave a thread the registers of its sums
+  static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 512), kMost = M == 16 ? 3 : 4;
+  static constexpr int kFit = kRoom < kMost ? kRoom : kMost;
+  static_assert(kWarps * M * kJoinPitch * 4 <= kStage, "the warps' triples meet in a stage");
+  static_assert(kRows * kChunks % kThreads == 0 && kRows <= kThreads, "");
 };
 
 // ----------------------------------------------------------------- the cache
@@ -188,35 +194,50 @@ __device__ __forceinline__ float ex2(float x) {
 
 // ------------------------------------------------------------------ the rows
 
-// One thread's share of a warp's 16 rows, as the matrix instructions lay an
-// accumulator out: rows g and g + 8, columns 8n + 2t and 8n + 2t + 1
-// (g = lane / 4, t = lane % 4).
-template <class T, int D>
+// One thread's share of a warp's M query rows (g = lane / 4, t = lane % 4).
+//
+// Scores are accumulators of (rows x keys): the thread holds rows g and, with
+// M = 16, g + 8, and of each eight keys 2t and 2t + 1.  With M <= 8 the second
+// half of the rows is zeros.
+//
+// Sums: with M = 16, or in 32 bits, (rows x dims) the same way: the thread's
+// rows, dims 8n + 2t and + 1.  With M <= 8 in 16 bits (dims x rows): dims 16n +
+// g and + 8, rows 2t and 2t + 1, so that no row of the product is empty; the
+// scores, turned over, are the second operand as they lie in the registers.
+// With M = 4 rows 4 to 7 repeat rows 0 to 3, and where the weights enter the
+// product as two 16-bit halves the repeated rows carry the low halves.
+template <class T, int D, int M>
 struct Rows {
-  uint32_t q[sizeof(T) == 2 ? D / 16 : 1][4];
-  float o[D / 8][4];
-  float m[2], z[2];
-  int end[2], low[2];  // visible: [low, end) and [0, sinks)
+  static constexpr int kOwn = M == 16 ? 2 : 1;                       // rows whose scores the thread holds
+  static constexpr bool kTurned = sizeof(T) == 2 && M <= 8;
+  static constexpr int kSums = kTurned ? D / 16 : D / 8, kEach = kTurned ? 4 : 2 * kOwn;
+  uint32_t q[sizeof(T) == 2 ? D / 16 : 1][2 * kOwn];
+  float o[kSums][kEach];
+  float m[kOwn], z[kOwn];
+  int end[kOwn], low[kOwn];  // visible: [low, end) and [0, sinks)
 };
 
-template <class T, int D>
+__device__ __forceinline__ int row_of(int lane, int M, int r) { return ((lane >> 2) & (M - 1)) + 8 * r; }
+
+template <class T>
 __device__ __forceinline__ const T* query_at(const Attend& p, int b, int head, int row) {
   const int i = (int)div_floor(row, p.groups), h = head * p.group + row - i * p.group;
   return (const T*)p.a.q + b * p.a.q_stride_req + i * p.a.q_stride_pos + h * p.a.q_stride_head;
 }
 
-// The queries of 16 rows from `row0` on (rows past the last one: zeros).
-template <class T, int D>
-__device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D>& w, const Cursor& c, int head, int row0,
+// The queries of M rows from `row0` on (rows past the last one: zeros).
+template <class T, int D, int M>
+__device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D, M>& w, const Cursor& c, int head, int row0,
                                            float* qs) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  using R = Rows<T, D, M>;
+  const int lane = threadIdx.x & 31, t = lane & 3;
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n)
+  for (int n = 0; n < R::kSums; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w.o[n][e] = 0.0f;
+    for (int e = 0; e < R::kEach; ++e) w.o[n][e] = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = row0 + g + 8 * r, i = (int)div_floor(row, p.groups);
+  for (int r = 0; r < R::kOwn; ++r) {
+    const int row = row0 + row_of(lane, M, r), i = (int)div_floor(row, p.groups);
     const int place = c.len - p.a.new_tokens + i;
     w.m[r] = -INFINITY;
     w.z[r] = 0.0f;
@@ -226,31 +247,33 @@ __device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D>& w, const
   }
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = row0 + g + 8 * r;
-      const T* q = query_at<T, D>(p, c.b, head, row);
+    for (int r = 0; r < R::kOwn; ++r) {
+      const int row = row0 + row_of(lane, M, r);
+      const T* q = query_at<T>(p, c.b, head, row);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          w.q[k][r + 2 * e] = row < p.rows ? *(const uint32_t*)(q + 16 * k + 8 * e + 2 * t) : 0u;
+          w.q[k][r + R::kOwn * e] =
+              row < p.rows ? *(const uint32_t*)(q + 16 * k + 8 * e + 2 * t) ^ p.negate : 0u;
     }
   } else {
     __syncwarp();
-    for (int x = lane; x < 16 * (D / 4); x += 32) {
+    for (int x = lane; x < M * (D / 4); x += 32) {
       const int r = x / (D / 4), d = x % (D / 4) * 4, row = row0 + r;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (row < p.rows) v = *(const float4*)(query_at<T, D>(p, c.b, head, row) + d);
+      if (row < p.rows) v = *(const float4*)(query_at<T>(p, c.b, head, row) + d);
+      if (p.negate) v = make_float4(-v.x, -v.y, -v.z, -v.w);
       *(float4*)(qs + r * (D + 4) + d) = v;
     }
     __syncwarp();
   }
 }
 
-// Scores of N/8 * 8 keys whose rows start at `keys`.
-template <class T, int D, int N>
-__device__ __forceinline__ void scores(const Rows<T, D>& w, float (&s)[N / 8][4], const char* keys, const float* qs) {
-  constexpr int kPitch = Shape<T, D>::kPitch;
+// Scores of N keys whose rows start at `keys`: s[n][2 r + e] is row r's, key 8n + 2t + e.
+template <class T, int D, int M, int N>
+__device__ __forceinline__ void scores(const Rows<T, D, M>& w, float (&s)[N / 8][4], const char* keys, const float* qs) {
+  constexpr int kPitch = Shape<T, D, M>::kPitch;
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int n = 0; n < N / 8; ++n)
@@ -259,26 +282,40 @@ __device__ __forceinline__ void scores(const Rows<T, D>& w, float (&s)[N / 8][4]
   if constexpr (sizeof(T) == 2) {
     const uint32_t at = smem_addr(keys) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + (lane >> 3 & 1) * 16;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k)
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t a[4];
+      if constexpr (M == 16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = w.q[k][e];
+      } else {
+        a[0] = w.q[k][0];
+        a[2] = w.q[k][1];
+        a[1] = a[3] = 0u;
+      }
 #pragma unroll
       for (int n = 0; n < N / 16; ++n) {
         uint32_t f[4];
         load_x4(f, at + n * 16 * kPitch + k * 32);
-        mma<T>(s[2 * n], w.q[k], f[0], f[1]);
-        mma<T>(s[2 * n + 1], w.q[k], f[2], f[3]);
+        mma<T>(s[2 * n], a, f[0], f[1]);
+        mma<T>(s[2 * n + 1], a, f[2], f[3]);
       }
+    }
   } else {
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2, t = lane & 3, row = row_of(lane, M, 0);
+    (void)g;
 #pragma unroll 2
     for (int d = 0; d < D; d += 4) {
-      const float4 q0 = *(const float4*)(qs + g * (D + 4) + d), q1 = *(const float4*)(qs + (g + 8) * (D + 4) + d);
+      const float4 q0 = *(const float4*)(qs + row * (D + 4) + d);
+      float4 q1 = q0;
+      if constexpr (M == 16) q1 = *(const float4*)(qs + (row + 8) * (D + 4) + d);
 #pragma unroll
       for (int n = 0; n < N / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float4 k = *(const float4*)(keys + (8 * n + 2 * t + e) * kPitch + d * 4);
           s[n][e] = fmaf(q0.w, k.w, fmaf(q0.z, k.z, fmaf(q0.y, k.y, fmaf(q0.x, k.x, s[n][e]))));
-          s[n][2 + e] = fmaf(q1.w, k.w, fmaf(q1.z, k.z, fmaf(q1.y, k.y, fmaf(q1.x, k.x, s[n][2 + e]))));
+          if constexpr (M == 16)
+            s[n][2 + e] = fmaf(q1.w, k.w, fmaf(q1.z, k.z, fmaf(q1.y, k.y, fmaf(q1.x, k.x, s[n][2 + e]))));
         }
     }
   }
@@ -290,69 +327,99 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t x, __nv_bfloat16) {
 __device__ __forceinline__ bool any_nonfinite(uint32_t x, __half) {
   return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
 }
+__device__ __forceinline__ bool any_nonfinite(uint32_t x, float) { return (x & 0x7f800000u) == 0x7f800000u; }
 
+template <int S, int E>
+struct Sums {
+  float o[S][E];
+};
 template <int N>
 struct Weights {
   float s[N / 8][4];
-  bool see[N / 8][4];
+  uint32_t see;  // bit 4n + e: s[n][e] is of a visible token
 };
 
 // o += s v with the weight 0 of a hidden token kept away from its value, which
 // may be anything: element by element.
-template <int D>
-struct Sums {
-  float o[D / 8][4];
-};
-template <class T, int D, int N>
-__device__ __noinline__ Sums<D> values_one_by_one(Sums<D> sums, Weights<N> weights, const char* vals) {
-  constexpr int kPitch = Shape<T, D>::kPitch;
-  auto& o = sums.o;
-  auto& s = weights.s;
-  auto& see = weights.see;
-  const int lane = threadIdx.x & 31, t = lane & 3;
+template <class T, int D, int M, int N>
+__device__ __noinline__ Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> values_one_by_one(
+    Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> sums, Weights<N> w, const char* vals) {
+  using R = Rows<T, D, M>;
+  constexpr int kPitch = Shape<T, D, M>::kPitch;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int n = 0; n < N / 8; ++n)
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int from = (lane & ~3) + x;  // the lane that holds columns 2x, 2x + 1 of these rows
-        const float p0 = __shfl_sync(~0u, s[n][e], from), p1 = __shfl_sync(~0u, s[n][2 + e], from);
-        const bool s0 = __shfl_sync(~0u, (int)see[n][e], from), s1 = __shfl_sync(~0u, (int)see[n][2 + e], from);
         const T* v = (const T*)(vals + (8 * n + 2 * x + e) * kPitch);
+        // the weights of the two rows that the thread's sums are of
+        float p[2];
+        bool see[2];
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
+        for (int r = 0; r < 2; ++r) {
+          const int from = R::kTurned ? ((2 * t + r) & (M - 1)) * 4 + x : (lane & ~3) + x;
+          const int slot = R::kTurned || M != 16 ? e : 2 * r + e;
+          p[r] = __shfl_sync(~0u, w.s[n][slot], from);
+          see[r] = __shfl_sync(~0u, w.see, from) >> (4 * n + slot) & 1;
+        }
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float f = to_f32(v[8 * d + 2 * t + c]);
-            if (s0) o[d][c] = fmaf(p0, f, o[d][c]);
-            if (s1) o[d][2 + c] = fmaf(p1, f, o[d][2 + c]);
+        for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+          for (int k = 0; k < R::kEach; ++k) {
+            if constexpr (R::kTurned) {
+              if (see[k & 1] && 2 * t < M) sums.o[d][k] = fmaf(p[k & 1], to_f32(v[16 * d + g + 8 * (k >> 1)]), sums.o[d][k]);
+            } else {
+              if (see[k >> 1]) sums.o[d][k] = fmaf(p[k >> 1], to_f32(v[8 * d + 2 * t + (k & 1)]), sums.o[d][k]);
+            }
           }
       }
   return sums;
 }
 
-// o += s v, the weights as sums of two 16-bit halves: one rounding of 2^-9 to
-// each weight would cost as much precision as the output's own.
-template <class T, int D, int N>
-__device__ __forceinline__ void values(float (&o)[D / 8][4], const float (&s)[N / 8][4], const char* vals) {
-  constexpr int kPitch = Shape<T, D>::kPitch;
+// o += s v.  In 16 bits the weights enter as sums of two halves: one rounding
+// of 2^-9 to each weight would cost as much precision as the output's own.
+template <class T, int D, int M, int N>
+__device__ __forceinline__ void values(Rows<T, D, M>& w, const float (&s)[N / 8][4], const char* vals) {
+  constexpr int kPitch = Shape<T, D, M>::kPitch;
   const int lane = threadIdx.x & 31;
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2 && M <= 8) {
+    // values (dims x keys) times weights (keys x rows)
+    const uint32_t at = smem_addr(vals) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + (lane >> 3 & 1) * 16;
+#pragma unroll
+    for (int n = 0; n < N / 16; ++n) {
+      uint32_t h0, h1, l0, l1;
+      split<T>(s[2 * n][0], s[2 * n][1], h0, l0);
+      split<T>(s[2 * n + 1][0], s[2 * n + 1][1], h1, l1);
+      if (M == 4 && lane >= 16) {
+        h0 = l0;
+        h1 = l1;
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t f[4];
+        load_x4_turned(f, at + n * 16 * kPitch + d * 32);
+        mma<T>(w.o[d], f, h0, h1);
+        if (M != 4) mma<T>(w.o[d], f, l0, l1);
+      }
+    }
+  } else if constexpr (sizeof(T) == 2) {
     const uint32_t at = smem_addr(vals) + (lane & 15) * kPitch + (lane >> 4) * 16;
 #pragma unroll
     for (int n = 0; n < N / 16; ++n) {
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) split<T>(s[2 * n + (e >> 1)][2 * (e & 1)], s[2 * n + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
+      for (int e = 0; e < 4; ++e)
+        split<T>(s[2 * n + (e >> 1)][2 * (e & 1)], s[2 * n + (e >> 1)][2 * (e & 1) + 1], hi[e], lo[e]);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         uint32_t f[4];
         load_x4_turned(f, at + n * 16 * kPitch + d * 32);
-        mma<T>(o[2 * d], hi, f[0], f[1]);
-        mma<T>(o[2 * d + 1], hi, f[2], f[3]);
-        mma<T>(o[2 * d], lo, f[0], f[1]);
-        mma<T>(o[2 * d + 1], lo, f[2], f[3]);
+        mma<T>(w.o[2 * d], hi, f[0], f[1]);
+        mma<T>(w.o[2 * d + 1], hi, f[2], f[3]);
+        mma<T>(w.o[2 * d], lo, f[0], f[1]);
+        mma<T>(w.o[2 * d + 1], lo, f[2], f[3]);
       }
     }
   } else {
@@ -364,110 +431,142 @@ __device__ __forceinline__ void values(float (&o)[D / 8][4], const float (&s)[N 
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int from = (lane & ~3) + x;
-          const float p0 = __shfl_sync(~0u, s[n][e], from), p1 = __shfl_sync(~0u, s[n][2 + e], from);
+          const float p0 = __shfl_sync(~0u, s[n][e], from);
+          float p1 = 0.0f;
+          if constexpr (M == 16) p1 = __shfl_sync(~0u, s[n][2 + e], from);
           const char* v = vals + (8 * n + 2 * x + e) * kPitch + 8 * t;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d) {
             const float2 f = *(const float2*)(v + 32 * d);
-            o[d][0] = fmaf(p0, f.x, o[d][0]);
-            o[d][1] = fmaf(p0, f.y, o[d][1]);
-            o[d][2] = fmaf(p1, f.x, o[d][2]);
-            o[d][3] = fmaf(p1, f.y, o[d][3]);
+            w.o[d][0] = fmaf(p0, f.x, w.o[d][0]);
+            w.o[d][1] = fmaf(p0, f.y, w.o[d][1]);
+            if constexpr (M == 16) {
+              w.o[d][2] = fmaf(p1, f.x, w.o[d][2]);
+              w.o[d][3] = fmaf(p1, f.y, w.o[d][3]);
+            }
           }
         }
   }
 }
 
 // One softmax step: N keys, the first of them token `j0`.  `mixed`: some row
-// may not see some of them (`known`: offsets of the keys, negative: no token).
-template <class T, int D, int N>
-__device__ __forceinline__ void step(const Attend& p, Rows<T, D>& w, const char* keys, const char* vals, const float* qs,
-                                     int j0, bool mixed, const int64_t* known) {
+// may not see some of them (`known`, from bit `bit0` on: the keys that are tokens).
+template <class T, int D, int M, int N>
+__device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const char* keys, const char* vals,
+                                     const float* qs, int j0, bool mixed, const uint32_t* known, int bit0) {
+  using R = Rows<T, D, M>;
   const int lane = threadIdx.x & 31, t = lane & 3;
   float s[N / 8][4];
-  scores<T, D, N>(w, s, keys, qs);
-  bool see[N / 8][4];
-#pragma unroll
-  for (int n = 0; n < N / 8; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
+  scores<T, D, M, N>(w, s, keys, qs);
+  uint32_t see = 0;
   if (mixed) {
     const int sinks = sinks_of(p);
 #pragma unroll
     for (int n = 0; n < N / 8; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = 8 * n + 2 * t + (e & 1), j = j0 + x, r = e >> 1;
-        see[n][e] = known[x] != -1 && j < w.end[r] && (j >= w.low[r] || j < sinks);
-        if (!see[n][e]) s[n][e] = -INFINITY;
+      for (int e = 0; e < 2 * R::kOwn; ++e) {
+        const int x = 8 * n + 2 * t + (e & 1), j = j0 + x, r = e >> 1, bit = bit0 + x;
+        const bool v = (known[bit >> 5] >> (bit & 31) & 1) && j < w.end[r] && (j >= w.low[r] || j < sinks);
+        see |= (uint32_t)v << (4 * n + e);
+        if (!v) s[n][e] = -INFINITY;
       }
   }
-  float top[2] = {-INFINITY, -INFINITY};
+  float fix[R::kOwn], base[R::kOwn];
+  bool moved = false;
 #pragma unroll
-  for (int n = 0; n < N / 8; ++n)
+  for (int r = 0; r < R::kOwn; ++r) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-  float fix[2], base[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 1));
-    top[r] = fmaxf(top[r], __shfl_xor_sync(~0u, top[r], 2));
-    const float m = fmaxf(w.m[r], top[r]);
+    for (int n = 0; n < N / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    const float m = fmaxf(w.m[r], top * p.scale_log2);  // the scale is not negative (see `negate`)
     base[r] = m == -INFINITY ? 0.0f : m;
     fix[r] = ex2(w.m[r] - base[r]);
+    moved |= fix[r] != 1.0f;
     w.m[r] = m;
   }
-  if (__any_sync(~0u, fix[0] != 1.0f || fix[1] != 1.0f)) {
+  if (__any_sync(~0u, moved)) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) w.z[r] *= fix[r];
+    for (int r = 0; r < R::kOwn; ++r) w.z[r] *= fix[r];
+    float f[2];  // of the rows that the thread's sums are of
+    if constexpr (R::kTurned) {
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
+      for (int r = 0; r < 2; ++r) f[r] = __shfl_sync(~0u, fix[0], ((2 * t + r) & (M - 1)) * 4);
+    } else {
+      f[0] = fix[0];
+      f[1] = fix[R::kOwn - 1];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w.o[d][e] *= fix[e >> 1];
+    for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+      for (int e = 0; e < R::kEach; ++e) w.o[d][e] *= f[R::kTurned ? e & 1 : e >> 1];
   }
 #pragma unroll
   for (int n = 0; n < N / 8; ++n)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[n][e] = ex2(s[n][e] - base[e >> 1]);
+    for (int e = 0; e < 2 * R::kOwn; ++e) {
+      s[n][e] = ex2(fmaf(s[n][e], p.scale_log2, -base[e >> 1]));
       w.z[e >> 1] += s[n][e];
     }
-  bool careful = false;
   if (mixed) {
     // a value that is not finite reaches only the rows that see its token
-    constexpr int kPitch = Shape<T, D>::kPitch;
-    for (int x = lane; x < N * (D * (int)sizeof(T) / 4); x += 32) {
-      const int r = x / (D * (int)sizeof(T) / 4), d = x % (D * (int)sizeof(T) / 4);
-      const uint32_t f = *(const uint32_t*)(vals + r * kPitch + 4 * d);
-      if constexpr (sizeof(T) == 2)
-        careful |= any_nonfinite(f, T());
-      else
-        careful |= (f & 0x7f800000u) == 0x7f800000u;
+    constexpr int kPitch = Shape<T, D, M>::kPitch, kPer = D * (int)sizeof(T) / 4;
+    bool careful = false;
+    for (int x = lane; x < N * kPer; x += 32)
+      careful |= any_nonfinite(*(const uint32_t*)(vals + x / kPer * kPitch + x % kPer * 4), T());
+    if (__any_sync(~0u, careful)) {
+      // by value: nothing of the common path has an address
+      Sums<R::kSums, R::kEach> sums;
+      Weights<N> weights;
+#pragma unroll
+      for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+        for (int e = 0; e < R::kEach; ++e) sums.o[d][e] = w.o[d][e];
+#pragma unroll
+      for (int n = 0; n < N / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) weights.s[n][e] = s[n][e];
+      weights.see = see;
+      sums = values_one_by_one<T, D, M, N>(sums, weights, vals);
+#pragma unroll
+      for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+        for (int e = 0; e < R::kEach; ++e) w.o[d][e] = sums.o[d][e];
+      return;
     }
-    careful = __any_sync(~0u, careful);
   }
-  if (careful) {
-    // by value: nothing of the common path has an address
-    Sums<D> sums;
-    Weights<N> weights;
+  values<T, D, M, N>(w, s, vals);
+}
+
+// A warp's triples to shared memory: maxima and sums by row, o by (row, dim).
+template <class T, int D, int M>
+__device__ __forceinline__ void put_rows(Rows<T, D, M>& w, float* ms, float* zs, float* joined) {
+  using R = Rows<T, D, M>;
+  constexpr int kJoin = Shape<T, D, M>::kJoinPitch;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
+  for (int r = 0; r < R::kOwn; ++r) {
+    w.z[r] += __shfl_xor_sync(~0u, w.z[r], 1);
+    w.z[r] += __shfl_xor_sync(~0u, w.z[r], 2);
+    if (t == 0 && g < M) {
+      ms[g + 8 * r] = w.m[r];
+      zs[g + 8 * r] = w.z[r];
+    }
+  }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums.o[d][e] = w.o[d][e];
-#pragma unroll
-    for (int n = 0; n < N / 8; ++n)
+  for (int d = 0; d < R::kSums; ++d) {
+    if constexpr (R::kTurned) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        weights.s[n][e] = s[n][e];
-        weights.see[n][e] = see[n][e];
+        if constexpr (M == 4) w.o[d][e] += __shfl_xor_sync(~0u, w.o[d][e], 2);
+        if (2 * t < M) joined[(2 * t + (e & 1)) * kJoin + 16 * d + g + 8 * (e >> 1)] = w.o[d][e];
       }
-    sums = values_one_by_one<T, D, N>(sums, weights, vals);
+    } else {
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w.o[d][e] = sums.o[d][e];
-  } else {
-    values<T, D, N>(w.o, s, vals);
+      for (int r = 0; r < R::kOwn; ++r)
+        if (g < M) *(float2*)(joined + (g + 8 * r) * kJoin + 8 * d + 2 * t) = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
+    }
   }
 }
 
@@ -530,22 +629,22 @@ __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int 
       z == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(z);
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ Attend p) {
-  using S = Shape<T, D>;
+template <class T, int D, int M>
+__global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(const __grid_constant__ Attend p) {
+  using S = Shape<T, D, M>;
   extern __shared__ __align__(128) char smem[];
   char* const ring = smem;
   float* const qs = (float*)(smem + S::kStages * S::kStage);
-  int64_t* const known = (int64_t*)(smem + S::kStages * S::kStage + S::kQ);  // [kStages + 1][kMaxKeys]
-  float* const ms = (float*)(known + (S::kStages + 1) * S::kMaxKeys);        // [kWarps][16], then z
-  float* const zs = ms + kWarps * 16;
-  __shared__ long long sums[kWarps + 1];
-  __shared__ int found[4];
+  int64_t* const places = (int64_t*)(qs + kWarps * S::kQuery);  // [2][kRows]
+  __shared__ uint32_t known[S::kStages + 1][S::kWords];  // which keys of a tile are tokens
+  __shared__ float ms[kWarps * M], zs[kWarps * M];       // maxima and sums that meet
+  __shared__ long long sums[kWarps];
+  __shared__ int found[3];
   __shared__ int arrived, bad;  // bad: some table entry so far is no page
 
   const yapd_cache& c = p.a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int shift = 31 - __clz(S::kRows / p.hg);  // keys of a tile, as a power of two
+  const int shift = 31 - __clz(S::kRows / p.hg), keys = 1 << shift;  // keys of a tile
   const int pairs = p.head_groups * p.row_blocks;
 
   // all units, and where this CTA's share begins
@@ -565,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     if (lane >= d) upto += y;
   }
   if (lane == 31) sums[warp] = upto;
+  if (tid == 0) bad = 0;
   __syncthreads();
   long long total = 0;
   for (int w = 0; w < kWarps; ++w) {
@@ -604,98 +704,98 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   }
 
   const long long units = u1 - u0;
-  Cursor get, put;  // the tile to be multiplied, the tile whose tokens are looked up
+  Cursor get, load, look;  // the tile that is multiplied, fetched, looked up
   get.b = found[0];
   get.hr = found[1];
   get.tile = found[2];
   if (units > 0) enter(p, get, shift);
-  put = get;
-  Cursor load = get;  // the tile to be fetched
+  load = look = get;
 
-  // the places of a tile's tokens: elements from the layer's start, -1: none,
-  // -2 - i: new token i, read from the call's rows
-  constexpr int kLook = S::kMaxKeys > kThreads ? S::kMaxKeys / kThreads : 1;
-  int page_of[kLook];
-  auto look = [&](const Cursor& x) {
-    const int k0 = tile_start(x, shift), low = first_low(p, x.len), sinks = sinks_of(p);
-#pragma unroll
-    for (int e = 0; e < kLook; ++e) {
-      const int j = k0 + tid + e * kThreads;
-      page_of[e] = INT32_MIN;  // no token
-      if (tid + e * kThreads < (1 << shift) && j < x.len && (j >= low || j < sinks)) {
-        page_of[e] = c.page_table[(int64_t)x.slot * c.max_pages + div_floor(j, p.page)];
-        if (page_of[e] == INT32_MIN) page_of[e] = -1;
+  // Looking a tile up is two halves, so that the read of the page table is on
+  // its way during a product: thread y holds key y's table entry, then notes the
+  // token's place, in elements from the layer's start (-1: no token, -2 - i: new
+  // token i, read from the call's rows).
+  constexpr int kNone = INT32_MIN;
+  int entry;
+  auto ask = [&](const Cursor& x) {
+    const int j = tile_start(x, shift) + tid, low = first_low(p, x.len), sinks = sinks_of(p);
+    entry = kNone;
+    if (tid < keys && j < x.len && (j >= low || j < sinks))
+      entry = max(c.page_table[(int64_t)x.slot * c.max_pages + div_floor(j, p.page)], -1);
+  };
+  auto note = [&](const Cursor& x, int tile) {
+    const int j = tile_start(x, shift) + tid, i = j - (x.len - p.a.new_tokens);
+    int64_t place = -1;
+    if (entry != kNone) {
+      if (p.a.k && i >= 0) {
+        place = -2 - i;
+      } else if (entry >= 0 && entry < c.pages) {
+        const int r = j - (int)div_floor(j, p.page) * c.page_size;
+        place = entry * c.stride_page + (int64_t)r * c.kv_heads * D;
+      } else {
+        bad = 1;
+        set_status(c.workspace, YAPD_STATUS_BAD_PAGE);
       }
     }
-  };
-  auto note = [&](const Cursor& x, int at) {
-    const int k0 = tile_start(x, shift);
-    bool wrong = false;
-#pragma unroll
-    for (int e = 0; e < kLook; ++e) {
-      const int y = tid + e * kThreads;
-      if (y >= (1 << shift)) break;
-      const int g = page_of[e], j = k0 + y, i = j - (x.len - p.a.new_tokens);
-      int64_t place = -1;
-      if (g != INT32_MIN) {
-        if (p.a.k && i >= 0) {
-          place = -2 - i;
-        } else if (g >= 0 && g < c.pages) {
-          const int r = j - (int)div_floor(j, p.page) * c.page_size;
-          place = g * c.stride_page + (int64_t)r * c.kv_heads * D;
-        } else {
-          wrong = true;
-        }
-      }
-      known[at * S::kMaxKeys + y] = place;
-    }
-    if (wrong) {
-      bad = 1;
-      set_status(c.workspace, YAPD_STATUS_BAD_PAGE);
+    if (tid < S::kRows) {
+      places[(tile & 1) * S::kRows + tid] = place;
+      const uint32_t mask = __ballot_sync(~0u, place != -1);
+      if (lane == 0) known[tile & S::kStages][warp] = mask;
     }
   };
-  auto fetch = [&](const Cursor& x, int stage, int at) {
+  static_assert(S::kStages == 3, "a ring of four masks");
+  const int64_t to_v = (int64_t)c.page_size * c.kv_heads * D;
+  auto fetch = [&](const Cursor& x, int stage, int tile) {
     const int head0 = x.hr / p.row_blocks * p.hg;
-    const T* base = (const T*)c.kv + p.a.layer * c.stride_layer;
-    const int64_t to_v = (int64_t)c.page_size * c.kv_heads * D;
+    const T* const base = (const T*)c.kv + p.a.layer * c.stride_layer + head0 * D;
+    const int64_t* const at = places + (tile & 1) * S::kRows;
     const uint32_t to = smem_addr(ring + stage * S::kStage);
-#pragma unroll 4
-    for (int e = 0; e < S::kLoads; ++e) {
-      const int y = tid + e * kThreads, row = y / S::kChunks, ch = y - row * S::kChunks;
-      const int kk = row & ((1 << shift) - 1), h = head0 + (row >> shift);
-      const int64_t place = known[at * S::kMaxKeys + kk];
-      const T* k = base + h * D;
-      const T* v = k;
-      if (place >= 0) {
-        k += place;
-        v = k + to_v;
-      } else if (place < -1) {
-        const int i = (int)(-2 - place);
-        k = (const T*)p.a.k + x.b * p.a.k_stride_req + i * p.a.k_stride_pos + h * p.a.k_stride_head;
-        v = (const T*)p.a.v + x.b * p.a.v_stride_req + i * p.a.v_stride_pos + h * p.a.v_stride_head;
+    constexpr int kVec = 16 / sizeof(T);
+    if (!p.a.k || tile_start(x, shift) + keys <= x.len - p.a.new_tokens) {
+#pragma unroll
+      for (int e = 0; e < S::kLoads; ++e) {
+        const int y = tid + e * kThreads, row = y / S::kChunks, ch = y - row * S::kChunks;
+        const int64_t place = at[row & (keys - 1)];
+        const T* const k = base + max(place, (int64_t)0) + (row >> shift) * D + ch * kVec;
+        const uint32_t d = to + row * S::kPitch + ch * 16;
+        copy16(d, k, place >= 0);
+        copy16(d + S::kHalf, k + to_v, place >= 0);
       }
-      const uint32_t d = to + row * S::kPitch + ch * 16;
-      copy16(d, k + ch * (16 / sizeof(T)), place != -1);
-      copy16(d + S::kHalf, v + ch * (16 / sizeof(T)), place != -1);
+    } else {
+      for (int e = 0; e < S::kLoads; ++e) {
+        const int y = tid + e * kThreads, row = y / S::kChunks, ch = y - row * S::kChunks, h = row >> shift;
+        const int64_t place = at[row & (keys - 1)];
+        const T *k = base, *v = base;
+        if (place >= 0) {
+          k = base + place + h * D + ch * kVec;
+          v = k + to_v;
+        } else if (place < -1) {
+          const int i = (int)(-2 - place);
+          k = (const T*)p.a.k + x.b * p.a.k_stride_req + i * p.a.k_stride_pos + (head0 + h) * p.a.k_stride_head + ch * kVec;
+          v = (const T*)p.a.v + x.b * p.a.v_stride_req + i * p.a.v_stride_pos + (head0 + h) * p.a.v_stride_head + ch * kVec;
+        }
+        const uint32_t d = to + row * S::kPitch + ch * 16;
+        copy16(d, k, place != -1);
+        copy16(d + S::kHalf, v, place != -1);
+      }
     }
   };
 
-  // the pipeline fills: tiles 0 .. kStages - 2 are under way, the next is looked up
-  if (tid == 0) bad = 0;
-  __syncthreads();
-  for (int s = 0; s < S::kStages; ++s)
+  // the pipeline fills: two tiles under way, the third looked up
+  for (int s = 0; s < S::kStages; ++s) {
     if (s < units) {
-      look(put);
-      note(put, s);
-      advance(p, put, shift);
+      ask(look);
+      note(look, s);
+      advance(p, look, shift);
     }
-  __syncthreads();
-  for (int s = 0; s < S::kStages - 1; ++s) {
-    if (s < units) {
-      fetch(load, s, s);
-      advance(p, load, shift);
+    __syncthreads();
+    if (s < S::kStages - 1) {
+      if (s < units) {
+        fetch(load, s, s);
+        advance(p, load, shift);
+      }
+      copies_commit();
     }
-    copies_commit();
   }
   if (p.a.k)
     for (int x = blockIdx.x; x < p.a.B * p.a.new_tokens; x += gridDim.x)
@@ -705,45 +805,43 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   const int span = S::kRows / wk_all;                    // stage rows of this warp
   const int parts = wk_all / p.hg;                       // warps that share a head's keys
   const int head_in = wk / parts, part = wk - head_in * parts;
-  float* const my_qs = qs + warp * 16 * (D + 4);
-  Rows<T, D> w;
+  float* const my_qs = qs + warp * S::kQuery;
+  Rows<T, D, M> w;
   bool fresh = true, whole = true;
+  int stage = 0;
   for (long long it = 0; it < units; ++it) {
     copies_wait<S::kStages - 2>();
     __syncthreads();
-    const int stage = (int)(it % S::kStages), at = (int)(it % (S::kStages + 1));
     if (it + S::kStages - 1 < units) {
-      fetch(load, (int)((it + S::kStages - 1) % S::kStages), (int)((it + S::kStages - 1) % (S::kStages + 1)));
+      fetch(load, stage == 0 ? S::kStages - 1 : stage - 1, (int)(it + S::kStages - 1));
       advance(p, load, shift);
     }
     copies_commit();
     const bool more = it + S::kStages < units;
-    if (more) look(put);
+    if (more) ask(look);
     const int head0 = get.hr / p.row_blocks * p.hg, rb = get.hr % p.row_blocks;
-    const int row0 = (rb * p.wr + wrow) * 16;
     if (fresh) {
       whole = get.tile == 0;
-      begin_rows<T, D>(p, w, get, head0 + head_in, row0, my_qs);
+      begin_rows<T, D, M>(p, w, get, head0 + head_in, (rb * p.wr + wrow) * M, my_qs);
       fresh = false;
     }
     {
-      const int k0 = tile_start(get, shift), keys = 1 << shift;
+      const int k0 = tile_start(get, shift);
       // every row sees every key of the tile
       const int first_end = p.a.causal ? get.len - p.a.new_tokens + 1 : get.len;
       const int64_t last_low = p.a.window > 0 ? (int64_t)get.len - p.a.window : 0;
       const bool mixed = bad || k0 + keys > first_end || (k0 < last_low && k0 + keys > p.a.sinks);
       const char* rows = ring + stage * S::kStage + wk * span * S::kPitch;
-      const int64_t* places = known + at * S::kMaxKeys + part * span;
       for (int x = 0; x < span; x += S::kStep) {
         const int j0 = k0 + part * span + x;
         if (j0 >= get.len) break;
-        step<T, D, S::kStep>(p, w, rows + x * S::kPitch, rows + S::kHalf + x * S::kPitch, my_qs, j0, mixed, places + x);
+        step<T, D, M, S::kStep>(p, w, rows + x * S::kPitch, rows + S::kHalf + x * S::kPitch, my_qs, j0, mixed,
+                                known[it & S::kStages], part * span + x);
       }
     }
     if (more) {
-      const int to = (int)((it + S::kStages) % (S::kStages + 1));
-      note(put, to);  // the place of tile it - 1: every warp has passed this iteration's barrier
-      advance(p, put, shift);
+      note(look, (int)(it + S::kStages));
+      advance(p, look, shift);
     }
     const bool last_tile = get.tile + 1 == get.span.tiles;
     if (last_tile || it + 1 == units) {
@@ -751,39 +849,24 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       whole = whole && last_tile;
       __syncthreads();
       float* const joined = (float*)(ring + stage * S::kStage);
-      {
-        const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          w.z[r] += __shfl_xor_sync(~0u, w.z[r], 1);
-          w.z[r] += __shfl_xor_sync(~0u, w.z[r], 2);
-          if (t == 0) {
-            ms[warp * 16 + g + 8 * r] = w.m[r];
-            zs[warp * 16 + g + 8 * r] = w.z[r];
-          }
-#pragma unroll
-          for (int d = 0; d < D / 8; ++d)
-            *(float2*)(joined + (warp * 16 + g + 8 * r) * S::kJoinPitch + 8 * d + 2 * t) =
-                make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
-        }
-      }
+      put_rows<T, D, M>(w, ms + warp * M, zs + warp * M, joined + warp * M * S::kJoinPitch);
       __syncthreads();
-      const int rows_here = min(p.wr * 16, p.rows - rb * p.wr * 16);
+      const int block_rows = p.wr * M, rows_here = min(block_rows, p.rows - rb * block_rows);
       // which CTAs hold parts of this (request, head group, row block)
       const long long u = u0 + it, start = u - get.tile, end = start + get.span.tiles;
-      const long long c0 = start / chunk, c1 = (end - 1) / chunk;
-      float* const mine_at =
-          p.partials + ((int64_t)blockIdx.x * 2 + (start > u0 ? 1 : 0)) * kMaxRows * (D + 2);
+      const int c0 = (int)(start / chunk), c1 = (int)((end - 1) / chunk);
+      constexpr int64_t kPart = kMaxRows * (D + 2);
+      float* const mine_at = p.partials + ((int64_t)blockIdx.x * 2 + (start > u0 ? 1 : 0)) * kPart;
       for (int x = tid; x < p.hg * rows_here * (D / 4); x += kThreads) {
         const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here, row = rr - hi * rows_here;
-        const int r16 = row & 15, first = (hi * parts) * p.wr + (row >> 4);
+        const int rm = row & (M - 1), first = (hi * parts) * p.wr + row / M;
         float m = -INFINITY;
-        for (int k = 0; k < parts; ++k) m = fmaxf(m, ms[(first + k * p.wr) * 16 + r16]);
+        for (int k = 0; k < parts; ++k) m = fmaxf(m, ms[(first + k * p.wr) * M + rm]);
         const float base = m == -INFINITY ? 0.0f : m;
         float z = 0.0f;
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int k = 0; k < parts; ++k) {
-          const int y = (first + k * p.wr) * 16 + r16;
+          const int y = (first + k * p.wr) * M + rm;
           const float f = ex2(ms[y] - base);
           const float4 v = *(const float4*)(joined + y * S::kJoinPitch + 4 * d);
           z = fmaf(f, zs[y], z);
@@ -794,10 +877,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         }
         if (whole) {
           const float rz = z == 0.0f ? 0.0f : 1.0f / z;
-          write_row<T>(p, get.b, head0 + hi, rb * p.wr * 16 + row, 4 * d, o, rz);
-          if (d == 0) write_lse(p, get.b, head0 + hi, rb * p.wr * 16 + row, m, z);
+          write_row<T>(p, get.b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
+          if (d == 0) write_lse(p, get.b, head0 + hi, rb * block_rows + row, m, z);
         } else {
-          float* const to = mine_at + (hi * rows_here + row) * (D + 2);
+          float* const to = mine_at + rr * (D + 2);
           *(float2*)(to + 4 * d) = make_float2(o.x, o.y);
           *(float2*)(to + 4 * d + 2) = make_float2(o.z, o.w);
           if (d == 0) *(float2*)(to + D) = make_float2(m, z);
@@ -807,83 +890,121 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         __threadfence();
         __syncthreads();
         if (tid == 0) {
-          const int n = (int)(c1 - c0) + 1, before = atomicAdd(p.counters + c0, 1);
-          arrived = before == n - 1;
+          const int before = atomicAdd(p.counters + c0, 1);
+          arrived = before == c1 - c0;
           if (arrived) p.counters[c0] = 0;  // for the next call; nobody else comes
         }
         __syncthreads();
         if (arrived) {
           __threadfence();
-          // CTA c0 left it in its second place unless the piece begins with it
-          const float* const from0 = p.partials + (c0 * 2 + (start > c0 * chunk ? 1 : 0)) * kMaxRows * (D + 2);
-          const float* const rest = p.partials + (c0 + 1) * 2 * kMaxRows * (D + 2);
-          const int n = (int)(c1 - c0);
-          for (int x = tid; x < p.hg * rows_here * (D / 2); x += kThreads) {
-            const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here, row = rr - hi * rows_here;
-            const float* const a = from0 + rr * (D + 2);
-            const float* const b = rest + rr * (D + 2);
-            float m = __ldcg(a + D);
-            for (int k = 0; k < n; ++k) m = fmaxf(m, __ldcg(b + (int64_t)k * 2 * kMaxRows * (D + 2) + D));
+          // the parts in their order: CTA c0's is its second unless its share begins with it
+          const int n = c1 - c0 + 1;
+          const float* const parts0 = p.partials + (c0 * 2 + (start > c0 * chunk ? 1 : 0)) * kPart;
+          const float* const parts1 = p.partials + (int64_t)c0 * 2 * kPart;
+          auto part_at = [&](int k) { return k == 0 ? parts0 : parts1 + k * 2 * kPart; };
+          // maxima and sums: a warp per row, lanes over the parts
+          for (int rr = warp; rr < p.hg * rows_here; rr += kWarps) {
+            float m = -INFINITY, z = 0.0f;
+            for (int k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(part_at(k) + rr * (D + 2) + D));
+#pragma unroll
+            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
             const float base = m == -INFINITY ? 0.0f : m;
-            float z = 0.0f;
+            for (int k = lane; k < n; k += 32) {
+              const float2 mz = __ldcg((const float2*)(part_at(k) + rr * (D + 2) + D));
+              z = fmaf(ex2(mz.x - base), mz.y, z);
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
+            if (lane == 0) {
+              const int hi = rr / rows_here;
+              ms[rr] = base;
+              zs[rr] = z == 0.0f ? 0.0f : 1.0f / z;
+              write_lse(p, get.b, head0 + hi, rb * block_rows + rr - hi * rows_here, m, z);
+            }
+          }
+          __syncthreads();
+          for (int x = tid; x < p.hg * rows_here * (D / 2); x += kThreads) {
+            const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here;
+            const float base = ms[rr], rz = zs[rr];
             float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 4
-            for (int k = -1; k < n; ++k) {
-              const float* const y = k < 0 ? a : b + (int64_t)k * 2 * kMaxRows * (D + 2);
-              const float2 mz = __ldcg((const float2*)(y + D)), v = __ldcg((const float2*)(y + 2 * d));
-              const float f = ex2(mz.x - base);
-              z = fmaf(f, mz.y, z);
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+              const float* const y = part_at(k) + rr * (D + 2);
+              const float f = ex2(__ldcg(y + D) - base);
+              const float2 v = __ldcg((const float2*)(y + 2 * d));
               o.x = fmaf(f, v.x, o.x);
               o.y = fmaf(f, v.y, o.y);
             }
-            const float rz = z == 0.0f ? 0.0f : 1.0f / z;
-            const int full = rb * p.wr * 16 + row, i = (int)div_floor(full, p.groups);
+            const int full = rb * block_rows + rr - hi * rows_here, i = (int)div_floor(full, p.groups);
             const int h = (head0 + hi) * p.group + full - i * p.group;
             T* const out = (T*)p.a.out + get.b * p.a.out_stride_req + i * p.a.out_stride_pos + h * p.a.out_stride_head + 2 * d;
             if constexpr (sizeof(T) == 4)
               *(float2*)out = make_float2(o.x * rz, o.y * rz);
             else
               *(uint32_t*)out = pack(from_f32<T>(o.x * rz), from_f32<T>(o.y * rz));
-            if (d == 0) write_lse(p, get.b, head0 + hi, full, m, z);
           }
         }
       }
       fresh = true;
     }
     advance(p, get, shift);
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
   }
 }
 
 // ------------------------------------------------------------------ the host
 
-template <class T, int D>
-int launch(Attend& p, cudaStream_t st) {
-  using S = Shape<T, D>;
-  int dev = 0, sms = 0, fit = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return YAPD_ERR_NO_DEVICE;
+// The kernel's grid on the current device: every CTA that fits at once.
+template <class T, int D, int M>
+int grid_of(int& grid) {
+  constexpr int kSmem = Shape<T, D, M>::kSmem;
   static std::atomic<int> grids[64];  // per device, found at its first call
-  if (dev >= 64) return YAPD_ERR_NO_DEVICE;
-  int grid = grids[dev].load(std::memory_order_relaxed);
-  if (!grid) {
-    if (cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, attend_kernel<T, D>, kThreads, S::kSmem) != cudaSuccess ||
-        fit < 1)
-      return YAPD_ERR_LAUNCH;
-    grid = sms * fit < kMaxCtas ? sms * fit : kMaxCtas;
-    grids[dev].store(grid, std::memory_order_relaxed);
-  }
-  attend_kernel<T, D><<<grid, kThreads, S::kSmem, st>>>(p);
+  int dev = 0, sms = 0, fit = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return YAPD_ERR_NO_DEVICE;
+  grid = grids[dev].load(std::memory_order_relaxed);
+  if (grid) return YAPD_OK;
+  if (cudaFuncSetAttribute(attend_kernel<T, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, attend_kernel<T, D, M>, kThreads, kSmem) != cudaSuccess ||
+      fit < 1)
+    return YAPD_ERR_LAUNCH;
+  grid = sms * fit < kMaxCtas ? sms * fit : kMaxCtas;
+  grids[dev].store(grid, std::memory_order_relaxed);
+  return YAPD_OK;
+}
+
+template <class T, int D, int M>
+int launch(Attend& p, cudaStream_t st) {
+  int grid = 0;
+  const int rc = grid_of<T, D, M>(grid);
+  if (rc != YAPD_OK) return rc;
+  p.wr = M < 16 || p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
+  p.row_blocks = (p.rows + M * p.wr - 1) / (M * p.wr);
+  // Key heads of a unit: the rows of several heads of a token lie side by side
+  // in its page.  Few requests are shared out by heads first, so that fewer
+  // CTAs hold parts of the same sums.
+  const int kvh = p.a.cache.kv_heads;
+  p.hg = 4 / p.wr;
+  while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < grid / 2)) p.hg /= 2;
+  p.head_groups = kvh / p.hg;
+  attend_kernel<T, D, M><<<grid, kThreads, Shape<T, D, M>::kSmem, st>>>(p);
   return launched();
+}
+
+template <class T, int D>
+int launch_rows(Attend& p, cudaStream_t st) {
+  if (sizeof(T) == 2 && p.rows <= 4) return launch<T, D, sizeof(T) == 2 ? 4 : 8>(p, st);
+  if (p.rows <= 8) return launch<T, D, 8>(p, st);
+  return launch<T, D, 16>(p, st);
 }
 
 template <class T>
 int launch_dim(Attend& p, cudaStream_t st) {
   switch (p.a.cache.head_dim) {
-    case 32: return launch<T, 32>(p, st);
-    case 64: return launch<T, 64>(p, st);
-    case 96: return launch<T, 96>(p, st);
-    default: return launch<T, 128>(p, st);
+    case 32: return launch_rows<T, 32>(p, st);
+    case 64: return launch_rows<T, 64>(p, st);
+    case 96: return launch_rows<T, 96>(p, st);
+    default: return launch_rows<T, 128>(p, st);
   }
 }
 
@@ -926,12 +1047,9 @@ extern "C" int yapd_attend(const yapd_attend_args* args, void* stream) {
   p.group = a.heads / kvh;
   p.groups = make_div((uint32_t)p.group);
   p.rows = a.new_tokens * p.group;
-  p.wr = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
-  p.row_blocks = (p.rows + 16 * p.wr - 1) / (16 * p.wr);
-  const int most = kWarps / p.wr;
-  p.hg = most >= 4 && kvh % 4 == 0 ? 4 : most >= 2 && kvh % 2 == 0 ? 2 : 1;
-  p.head_groups = kvh / p.hg;
-  p.scale_log2 = a.scale * 1.4426950408889634f;
+  // a negative scale is a positive one of the negative queries
+  p.negate = std::signbit(a.scale) ? dt == YAPD_DTYPE_F32 ? 0x80000000u : 0x80008000u : 0u;
+  p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
   char* const scratch = (char*)a.cache.workspace + kHeaderBytes + pages_scratch_bytes(a.cache);
   p.counters = (int*)scratch;
   p.partials = (float*)(scratch + round_up(kMaxCtas * 4, 256));
