@@ -109,6 +109,9 @@ typedef struct yapd_attend_args {
   float scale;
   int32_t causal;
   int64_t window, sinks;        /* window <= 0: no window */
+  int64_t wait_limit_ns;        /* as in yapd_select_args; a request whose keys
+                                   did not arrive has no or NaN outputs, and
+                                   YAPD_STATUS_WAIT_TIMEOUT is set */
 } yapd_attend_args;
 
 int yapd_attend(const yapd_attend_args* args, void* stream);

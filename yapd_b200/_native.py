@@ -144,7 +144,7 @@ class AttendArgs(C.Structure):
         ("out", C.c_void_p), ("out_stride_req", C.c_int64), ("out_stride_pos", C.c_int64),
         ("out_stride_head", C.c_int64),
         ("lse", C.c_void_p), ("scale", C.c_float), ("causal", C.c_int32),
-        ("window", C.c_int64), ("sinks", C.c_int64),
+        ("window", C.c_int64), ("sinks", C.c_int64), ("wait_limit_ns", C.c_int64),
     ]
 
 

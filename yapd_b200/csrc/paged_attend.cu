@@ -12,17 +12,22 @@
 // holds whole is written by it; one that is cut leaves a triple per CTA in the
 // workspace, and the CTA that arrives last joins them in their order.  No CTA
 // waits for another one.
+#include <cuda.h>  // CUtensorMap and the encode signature (the driver is reached at run time)
+
 #include <atomic>
 #include <cmath>
+#include <mutex>
 
+#include "select_common.cuh"
 #include "serve_common.cuh"
 
 namespace serve {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 4;                     // that multiply; one more fetches
+constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kMaxRows = 64;  // query rows times key heads of a unit at most
+constexpr int64_t kWaitNs = 500000000;
 
 struct Attend {
   yapd_attend_args a;
@@ -33,8 +38,10 @@ struct Attend {
   int wr;            // warps along the rows: 1, 2, 4 (1 unless M = 16)
   int hg;            // key heads of a unit: 1, 2, 4
   int head_groups, row_blocks;
+  bool boxes;        // pages are whole groups of 16 tokens
   uint32_t negate;   // sign bits of the queries to turn
   float scale_log2;  // not negative
+  int64_t wait_ns;   // limit of each wait
   int* counters;     // (gridDim): arrivals at a cut piece that starts in the CTA
   float* partials;   // (gridDim, 2, kMaxRows, D + 2)
 };
@@ -42,26 +49,35 @@ struct Attend {
 // ------------------------------------------------------------ shapes by type
 
 // M: query rows of a warp, 4, 8 or 16.
+//
+// A stage holds the keys, then the values, of a tile: groups of 16 tokens, in a
+// group a slab for each 128 (64) bytes of the head dimension of each head, in a
+// slab a row for each token. The 16-byte chunks of a row are permuted by the
+// token (swizzle), so that the same chunk of eight tokens lies in eight
+// different banks; it is the layout that a tensor copy of a group writes.
 template <class T, int D, int M>
 struct Shape {
-  // rows of keys in a stage, and as many of values
-  static constexpr int kRows = sizeof(T) == 2 ? (D == 32 ? 128 : 64) : (D == 32 ? 64 : 32);
+  static constexpr int kRows = sizeof(T) == 2 ? (D == 32 ? 128 : 64) : (D == 32 ? 64 : 32);  // tokens x heads of a stage
   static constexpr int kStep = kRows / kWarps < 32 ? kRows / kWarps : 32;  // keys of one softmax step
-  static constexpr int kPitch = D * sizeof(T) + 16;  // bytes: eight rows' 16-byte chunks fall in different banks
-  static constexpr int kHalf = kRows * kPitch;
+  static constexpr int kBytes = D * (int)sizeof(T);
+  static constexpr int kInner = kBytes % 128 == 0 ? 128 : 64;  // bytes of a row
+  static constexpr int kSlabs = kBytes / kInner;               // of a head
+  static constexpr int kSlab = 16 * kInner;
+  static constexpr int kHalf = kRows * kBytes;
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kStages = 3;
-  static constexpr int kChunks = D * sizeof(T) / 16;
-  static constexpr int kLoads = kRows * kChunks / kThreads;
-  static constexpr int kJoinPitch = D + 4;           // floats
-  static constexpr int kWords = kRows / 32;          // of a mask of keys
+  static constexpr int kMaxHeads = kRows / 16 < kWarps ? kRows / 16 : kWarps;  // key heads of a tile
+  static constexpr int kJoinPitch = D;               // floats
+  static constexpr int kWords = kRows / 32;          // of a mask of a tile's keys
   static constexpr int kQuery = sizeof(T) == 4 ? M * (D + 4) : 0;  // floats of a warp's queries in shared memory
-  static constexpr int kSmem = kStages * kStage + kWarps * kQuery * 4 + 2 * kRows * 8;
+  static constexpr int kSmem = kStages * kStage + kWarps * kQuery * 4;
   // CTAs of an SM: as many as its 228 KB hold, and no more than leave a thread the registers of its sums
-  static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 512), kMost = M == 16 ? 3 : 4;
+  static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 1024), kMost = M == 16 ? 3 : 4;
   static constexpr int kFit = kRoom < kMost ? kRoom : kMost;
   static_assert(kWarps * M * kJoinPitch * 4 <= kStage, "the warps' triples meet in a stage");
-  static_assert(kRows * kChunks % kThreads == 0 && kRows <= kThreads, "");
+
+  // Where 16-byte chunk `ch` of a row lies: token `tok` (of 16).
+  __device__ static __forceinline__ int turn(int tok) { return (kInner == 128 ? tok & 7 : tok >> 1 & 3) << 4; }
 };
 
 // ----------------------------------------------------------------- the cache
@@ -125,19 +141,24 @@ __device__ __forceinline__ int tile_start(const Cursor& c, int shift) {
   return (c.tile < c.span.sink_tiles ? c.tile : c.tile + c.span.skip) << shift;
 }
 
-// ------------------------------------------------------------------- copies
-
 __device__ __forceinline__ uint32_t smem_addr(const void* x) { return (uint32_t)__cvta_generic_to_shared(x); }
 
 // 16 bytes to shared memory, or zeros where `from` is not to be read.
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(read ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A box of 16 tokens of one page, all slabs of the unit's heads.
+__device__ __forceinline__ void copy_group(uint32_t to, const CUtensorMap* map, uint64_t* bar, int token, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %3, %6}], [%2];" ::"r"(to),
+      "l"(map), "r"(smem_addr(bar)), "r"(0), "r"(token), "r"(head), "r"(page)
+      : "memory");
 }
+// Arrives at `bar` when all earlier copies of this thread have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // ------------------------------------------------------------ matrix products
 
@@ -170,20 +191,28 @@ __device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t pack(__nv_bfloat16 lo, __nv_bfloat16 hi) {
-  __nv_bfloat162 x(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&x);
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
-__device__ __forceinline__ uint32_t pack(__half lo, __half hi) {
-  __half2 x(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&x);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 x = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
+__device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t x, __half) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
 // x and y as the sums of two T each
 template <class T>
 __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t& low) {
-  const T hx = from_f32<T>(x), hy = from_f32<T>(y);
-  high = pack(hx, hy);
-  low = pack(from_f32<T>(x - to_f32(hx)), from_f32<T>(y - to_f32(hy)));
+  high = pack2<T>(x, y);
+  const float2 h = unpack2(high, T());
+  low = pack2<T>(x - h.x, y - h.y);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -270,17 +299,26 @@ __device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D, M>& w, co
   }
 }
 
-// Scores of N keys whose rows start at `keys`: s[n][2 r + e] is row r's, key 8n + 2t + e.
+// Where a warp's keys lie in a stage, and how the layout goes on.
+struct Place {
+  const char* keys;  // the group's first slab of the warp's head
+  int first;         // token of the group that a step begins with
+  int slab;          // bytes between the slabs of a head
+  int group;         // bytes between groups
+};
+
+// Scores of N keys: s[n][2 r + e] is row r's, key 8n + 2t + e.
 template <class T, int D, int M, int N>
-__device__ __forceinline__ void scores(const Rows<T, D, M>& w, float (&s)[N / 8][4], const char* keys, const float* qs) {
-  constexpr int kPitch = Shape<T, D, M>::kPitch;
+__device__ __forceinline__ void scores(const Rows<T, D, M>& w, float (&s)[N / 8][4], const Place& at, const float* qs) {
+  using S = Shape<T, D, M>;
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int n = 0; n < N / 8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
   if constexpr (sizeof(T) == 2) {
-    const uint32_t at = smem_addr(keys) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + (lane >> 3 & 1) * 16;
+    const int tok = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t row = smem_addr(at.keys) + tok * S::kInner + ((lane >> 3 & 1) << 4 ^ S::turn(tok));
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
       uint32_t a[4];
@@ -292,27 +330,29 @@ __device__ __forceinline__ void scores(const Rows<T, D, M>& w, float (&s)[N / 8]
         a[2] = w.q[k][1];
         a[1] = a[3] = 0u;
       }
+      constexpr int kIn = S::kInner / 32;  // products of a slab
 #pragma unroll
       for (int n = 0; n < N / 16; ++n) {
         uint32_t f[4];
-        load_x4(f, at + n * 16 * kPitch + k * 32);
+        load_x4(f, ((row + k / kIn * at.slab) ^ (k % kIn << 5)) + n * at.group);
         mma<T>(s[2 * n], a, f[0], f[1]);
         mma<T>(s[2 * n + 1], a, f[2], f[3]);
       }
     }
   } else {
-    const int g = lane >> 2, t = lane & 3, row = row_of(lane, M, 0);
-    (void)g;
+    const int t = lane & 3, row = row_of(lane, M, 0);
 #pragma unroll 2
     for (int d = 0; d < D; d += 4) {
       const float4 q0 = *(const float4*)(qs + row * (D + 4) + d);
       float4 q1 = q0;
       if constexpr (M == 16) q1 = *(const float4*)(qs + (row + 8) * (D + 4) + d);
+      const char* const slab = at.keys + d / 32 * at.slab;
 #pragma unroll
       for (int n = 0; n < N / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float4 k = *(const float4*)(keys + (8 * n + 2 * t + e) * kPitch + d * 4);
+          const int tok = at.first + 8 * n + 2 * t + e;
+          const float4 k = *(const float4*)(slab + tok * S::kInner + (d % 32 * 4 ^ S::turn(tok)));
           s[n][e] = fmaf(q0.w, k.w, fmaf(q0.z, k.z, fmaf(q0.y, k.y, fmaf(q0.x, k.x, s[n][e]))));
           if constexpr (M == 16)
             s[n][2 + e] = fmaf(q1.w, k.w, fmaf(q1.z, k.z, fmaf(q1.y, k.y, fmaf(q1.x, k.x, s[n][2 + e]))));
@@ -321,13 +361,28 @@ __device__ __forceinline__ void scores(const Rows<T, D, M>& w, float (&s)[N / 8]
   }
 }
 
-__device__ __forceinline__ bool any_nonfinite(uint32_t x, __nv_bfloat16) {
-  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+template <class T>
+__device__ __forceinline__ bool finite_half(uint32_t x);
+template <>
+__device__ __forceinline__ bool finite_half<__nv_bfloat16>(uint32_t x) { return (x & 0x7f80u) != 0x7f80u; }
+template <>
+__device__ __forceinline__ bool finite_half<__half>(uint32_t x) { return (x & 0x7c00u) != 0x7c00u; }
+template <class T>
+__device__ __forceinline__ bool finite_word(uint32_t x) {
+  if constexpr (sizeof(T) == 4)
+    return (x & 0x7f800000u) != 0x7f800000u;
+  else
+    return finite_half<T>(x & 0xffffu) && finite_half<T>(x >> 16);
 }
-__device__ __forceinline__ bool any_nonfinite(uint32_t x, __half) {
-  return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u;
+
+// Where element `d` of key `x` of a step lies, in the keys' or the values' half.
+template <class T, int D, int M>
+__device__ __forceinline__ const T* element_at(const Place& at, const char* half, int x, int d) {
+  using S = Shape<T, D, M>;
+  const int y = at.first + x, tok = y & 15, byte = d * (int)sizeof(T);
+  return (const T*)(half + (y >> 4) * at.group + byte / S::kInner * at.slab + tok * S::kInner +
+                    (byte % S::kInner ^ S::turn(tok)));
 }
-__device__ __forceinline__ bool any_nonfinite(uint32_t x, float) { return (x & 0x7f800000u) == 0x7f800000u; }
 
 template <int S, int E>
 struct Sums {
@@ -339,54 +394,29 @@ struct Weights {
   uint32_t see;  // bit 4n + e: s[n][e] is of a visible token
 };
 
-// o += s v with the weight 0 of a hidden token kept away from its value, which
-// may be anything: element by element.
-template <class T, int D, int M, int N>
-__device__ __noinline__ Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> values_one_by_one(
-    Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> sums, Weights<N> w, const char* vals) {
-  using R = Rows<T, D, M>;
-  constexpr int kPitch = Shape<T, D, M>::kPitch;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// Zeros in the place of what is not finite.
+template <class T>
+__device__ __forceinline__ void clean(uint32_t (&f)[4]) {
 #pragma unroll
-  for (int n = 0; n < N / 8; ++n)
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const T* v = (const T*)(vals + (8 * n + 2 * x + e) * kPitch);
-        // the weights of the two rows that the thread's sums are of
-        float p[2];
-        bool see[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int from = R::kTurned ? ((2 * t + r) & (M - 1)) * 4 + x : (lane & ~3) + x;
-          const int slot = R::kTurned || M != 16 ? e : 2 * r + e;
-          p[r] = __shfl_sync(~0u, w.s[n][slot], from);
-          see[r] = __shfl_sync(~0u, w.see, from) >> (4 * n + slot) & 1;
-        }
-#pragma unroll
-        for (int d = 0; d < R::kSums; ++d)
-#pragma unroll
-          for (int k = 0; k < R::kEach; ++k) {
-            if constexpr (R::kTurned) {
-              if (see[k & 1] && 2 * t < M) sums.o[d][k] = fmaf(p[k & 1], to_f32(v[16 * d + g + 8 * (k >> 1)]), sums.o[d][k]);
-            } else {
-              if (see[k >> 1]) sums.o[d][k] = fmaf(p[k >> 1], to_f32(v[8 * d + 2 * t + (k & 1)]), sums.o[d][k]);
-            }
-          }
-      }
-  return sums;
+  for (int e = 0; e < 4; ++e) {
+    if (!finite_half<T>(f[e] & 0xffffu)) f[e] &= 0xffff0000u;
+    if (!finite_half<T>(f[e] >> 16)) f[e] &= 0xffffu;
+  }
 }
 
-// o += s v.  In 16 bits the weights enter as sums of two halves: one rounding
+// o += s v, with kClean only the finite values.  In 16 bits the weights enter as sums of two halves: one rounding
 // of 2^-9 to each weight would cost as much precision as the output's own.
-template <class T, int D, int M, int N>
-__device__ __forceinline__ void values(Rows<T, D, M>& w, const float (&s)[N / 8][4], const char* vals) {
-  constexpr int kPitch = Shape<T, D, M>::kPitch;
+template <class T, int D, int M, int N, bool kClean>
+__device__ __forceinline__ void values(float (&o)[Rows<T, D, M>::kSums][Rows<T, D, M>::kEach], const float (&s)[N / 8][4],
+                                       const Place& at) {
+  using S = Shape<T, D, M>;
   const int lane = threadIdx.x & 31;
+  const char* const vals = at.keys + S::kHalf;
+  constexpr int kIn = S::kInner / 32;  // 16 dims of a slab
   if constexpr (sizeof(T) == 2 && M <= 8) {
     // values (dims x keys) times weights (keys x rows)
-    const uint32_t at = smem_addr(vals) + ((lane >> 4) * 8 + (lane & 7)) * kPitch + (lane >> 3 & 1) * 16;
+    const int tok = (lane >> 4) * 8 + (lane & 7);
+    const uint32_t row = smem_addr(vals) + tok * S::kInner + ((lane >> 3 & 1) << 4 ^ S::turn(tok));
 #pragma unroll
     for (int n = 0; n < N / 16; ++n) {
       uint32_t h0, h1, l0, l1;
@@ -399,13 +429,15 @@ __device__ __forceinline__ void values(Rows<T, D, M>& w, const float (&s)[N / 8]
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         uint32_t f[4];
-        load_x4_turned(f, at + n * 16 * kPitch + d * 32);
-        mma<T>(w.o[d], f, h0, h1);
-        if (M != 4) mma<T>(w.o[d], f, l0, l1);
+        load_x4_turned(f, ((row + d / kIn * at.slab) ^ (d % kIn << 5)) + n * at.group);
+        if (kClean) clean<T>(f);
+        mma<T>(o[d], f, h0, h1);
+        if (M != 4) mma<T>(o[d], f, l0, l1);
       }
     }
   } else if constexpr (sizeof(T) == 2) {
-    const uint32_t at = smem_addr(vals) + (lane & 15) * kPitch + (lane >> 4) * 16;
+    const int tok = lane & 15;
+    const uint32_t row = smem_addr(vals) + tok * S::kInner + ((lane >> 4) << 4 ^ S::turn(tok));
 #pragma unroll
     for (int n = 0; n < N / 16; ++n) {
       uint32_t hi[4], lo[4];
@@ -415,11 +447,12 @@ __device__ __forceinline__ void values(Rows<T, D, M>& w, const float (&s)[N / 8]
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         uint32_t f[4];
-        load_x4_turned(f, at + n * 16 * kPitch + d * 32);
-        mma<T>(w.o[2 * d], hi, f[0], f[1]);
-        mma<T>(w.o[2 * d + 1], hi, f[2], f[3]);
-        mma<T>(w.o[2 * d], lo, f[0], f[1]);
-        mma<T>(w.o[2 * d + 1], lo, f[2], f[3]);
+        load_x4_turned(f, ((row + d / kIn * at.slab) ^ (d % kIn << 5)) + n * at.group);
+        if (kClean) clean<T>(f);
+        mma<T>(o[2 * d], hi, f[0], f[1]);
+        mma<T>(o[2 * d + 1], hi, f[2], f[3]);
+        mma<T>(o[2 * d], lo, f[0], f[1]);
+        mma<T>(o[2 * d + 1], lo, f[2], f[3]);
       }
     }
   } else {
@@ -434,30 +467,74 @@ __device__ __forceinline__ void values(Rows<T, D, M>& w, const float (&s)[N / 8]
           const float p0 = __shfl_sync(~0u, s[n][e], from);
           float p1 = 0.0f;
           if constexpr (M == 16) p1 = __shfl_sync(~0u, s[n][2 + e], from);
-          const char* v = vals + (8 * n + 2 * x + e) * kPitch + 8 * t;
+          const int tok = at.first + 8 * n + 2 * x + e;
+          const char* const v = vals + tok * S::kInner;
 #pragma unroll
           for (int d = 0; d < D / 8; ++d) {
-            const float2 f = *(const float2*)(v + 32 * d);
-            w.o[d][0] = fmaf(p0, f.x, w.o[d][0]);
-            w.o[d][1] = fmaf(p0, f.y, w.o[d][1]);
+            float2 f = *(const float2*)(v + d / 4 * at.slab + ((d % 4 * 32 + t * 8) ^ S::turn(tok)));
+            if (kClean) {
+              if (!isfinite(f.x)) f.x = 0.0f;
+              if (!isfinite(f.y)) f.y = 0.0f;
+            }
+            o[d][0] = fmaf(p0, f.x, o[d][0]);
+            o[d][1] = fmaf(p0, f.y, o[d][1]);
             if constexpr (M == 16) {
-              w.o[d][2] = fmaf(p1, f.x, w.o[d][2]);
-              w.o[d][3] = fmaf(p1, f.y, w.o[d][3]);
+              o[d][2] = fmaf(p1, f.x, o[d][2]);
+              o[d][3] = fmaf(p1, f.y, o[d][3]);
             }
           }
         }
   }
 }
 
+// o += s v where a value is not finite: the weight 0 of a token that a row does
+// not see must not meet it. The finite ones as ever, then the others one by one,
+// for the rows that see them.
+template <class T, int D, int M, int N>
+__device__ __noinline__ Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> values_with_care(
+    Sums<Rows<T, D, M>::kSums, Rows<T, D, M>::kEach> sums, Weights<N> w, Place at) {
+  using R = Rows<T, D, M>;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  values<T, D, M, N, true>(sums.o, w.s, at);
+  const char* const vals = at.keys + Shape<T, D, M>::kHalf;
+#pragma unroll
+  for (int n = 0; n < N / 8; ++n)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = 8 * n + 2 * x + e;
+        // the weights of the two rows that the thread's sums are of
+        float p[2];
+        bool see[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int from = R::kTurned ? ((2 * t + r) & (M - 1)) * 4 + x : (lane & ~3) + x;
+          const int slot = R::kTurned || M != 16 ? e : 2 * r + e;
+          p[r] = __shfl_sync(~0u, w.s[n][slot], from);
+          see[r] = __shfl_sync(~0u, w.see, from) >> (4 * n + slot) & 1;
+        }
+#pragma unroll
+        for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+          for (int k = 0; k < R::kEach; ++k) {
+            const int r = R::kTurned ? k & 1 : k >> 1, dim = R::kTurned ? 16 * d + g + 8 * (k >> 1) : 8 * d + 2 * t + (k & 1);
+            const float f = to_f32(*element_at<T, D, M>(at, vals, key, dim));
+            if (!isfinite(f) && see[r]) sums.o[d][k] = fmaf(p[r], f, sums.o[d][k]);
+          }
+      }
+  return sums;
+}
+
 // One softmax step: N keys, the first of them token `j0`.  `mixed`: some row
 // may not see some of them (`known`, from bit `bit0` on: the keys that are tokens).
 template <class T, int D, int M, int N>
-__device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const char* keys, const char* vals,
-                                     const float* qs, int j0, bool mixed, const uint32_t* known, int bit0) {
+__device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Place& at, const float* qs, int j0,
+                                     bool mixed, const uint32_t* known, int bit0) {
   using R = Rows<T, D, M>;
   const int lane = threadIdx.x & 31, t = lane & 3;
   float s[N / 8][4];
-  scores<T, D, M, N>(w, s, keys, qs);
+  scores<T, D, M, N>(w, s, at, qs);
   uint32_t see = 0;
   if (mixed) {
     const int sinks = sinks_of(p);
@@ -511,10 +588,11 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const ch
     }
   if (mixed) {
     // a value that is not finite reaches only the rows that see its token
-    constexpr int kPitch = Shape<T, D, M>::kPitch, kPer = D * (int)sizeof(T) / 4;
+    constexpr int kPer = D * (int)sizeof(T) / 4, kEl = 4 / (int)sizeof(T);
+    const char* const vals = at.keys + Shape<T, D, M>::kHalf;
     bool careful = false;
     for (int x = lane; x < N * kPer; x += 32)
-      careful |= any_nonfinite(*(const uint32_t*)(vals + x / kPer * kPitch + x % kPer * 4), T());
+      careful |= !finite_word<T>(*(const uint32_t*)element_at<T, D, M>(at, vals, x / kPer, x % kPer * kEl));
     if (__any_sync(~0u, careful)) {
       // by value: nothing of the common path has an address
       Sums<R::kSums, R::kEach> sums;
@@ -528,7 +606,7 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const ch
 #pragma unroll
         for (int e = 0; e < 4; ++e) weights.s[n][e] = s[n][e];
       weights.see = see;
-      sums = values_one_by_one<T, D, M, N>(sums, weights, vals);
+      sums = values_with_care<T, D, M, N>(sums, weights, at);
 #pragma unroll
       for (int d = 0; d < R::kSums; ++d)
 #pragma unroll
@@ -536,7 +614,7 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const ch
       return;
     }
   }
-  values<T, D, M, N>(w, s, vals);
+  values<T, D, M, N, false>(w.o, s, at);
 }
 
 // A warp's triples to shared memory: maxima and sums by row, o by (row, dim).
@@ -600,7 +678,7 @@ __device__ void store_token(const Attend& p, int b, int i) {
   const int per = c.head_dim / kVec, all = c.kv_heads * per;
   T* to = (T*)c.kv + p.a.layer * c.stride_layer + g * c.stride_page + (int64_t)(t - q * c.page_size) * c.kv_heads * c.head_dim;
   T* to_v = to + (int64_t)c.page_size * c.kv_heads * c.head_dim;
-  for (int x = threadIdx.x; x < all; x += kThreads) {
+  for (int x = threadIdx.x; x < all; x += kWarps * 32) {
     const int h = x / per, d = (x - h * per) * kVec;
     const uint4 k = *(const uint4*)((const T*)p.a.k + b * p.a.k_stride_req + i * p.a.k_stride_pos + h * p.a.k_stride_head + d);
     const uint4 v = *(const uint4*)((const T*)p.a.v + b * p.a.v_stride_req + i * p.a.v_stride_pos + h * p.a.v_stride_head + d);
@@ -617,8 +695,8 @@ __device__ __forceinline__ void write_row(const Attend& p, int b, int head, int 
     *(float4*)out = make_float4(o.x * rz, o.y * rz, o.z * rz, o.w * rz);
   } else {
     uint2 x;
-    x.x = pack(from_f32<T>(o.x * rz), from_f32<T>(o.y * rz));
-    x.y = pack(from_f32<T>(o.z * rz), from_f32<T>(o.w * rz));
+    x.x = pack2<T>(o.x * rz, o.y * rz);
+    x.y = pack2<T>(o.z * rz, o.w * rz);
     *(uint2*)out = x;
   }
 }
@@ -629,23 +707,55 @@ __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int 
       z == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(z);
 }
 
+// What the fetching warp says of a tile.
+struct Tile {
+  int b, head0, rb, len, k0;  // request, first key head, row block, tokens, first token
+  int tile, tiles;            // of the piece
+  bool mixed, last;  // some row may not see some key; the share's or the piece's last tile
+};
+
 template <class T, int D, int M>
-__global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(const __grid_constant__ Attend p) {
+struct Shared {
   using S = Shape<T, D, M>;
-  extern __shared__ __align__(128) char smem[];
+  uint64_t full[S::kStages], empty[S::kStages], met;
+  Tile tile[S::kStages];
+  uint32_t known[S::kStages][S::kWords];   // which keys of a tile are tokens
+  float m[kWarps * M], z[kWarps * M];      // maxima and sums that meet
+  long long sums[kThreads / 32];
+  int found[3];
+  int arrived, given_up;
+  int left;  // pieces of the share left for others to join: 1 the first, 2 the last
+};
+
+// Of a piece cut by the CTAs' shares of `chunk` units, [start, end): the first
+// CTA that holds some of it, how many do, and where each left its triples. The
+// first one's share may begin with another piece, whose place is the other one.
+struct Cut {
+  int c0, n, off;
+  __device__ Cut(long long start, long long end, long long chunk) {
+    c0 = (int)(start / chunk);
+    n = (int)((end - 1) / chunk) - c0 + 1;
+    off = start > c0 * chunk;
+  }
+  template <int kPart>
+  __device__ const float* part(const float* partials, int k) const {
+    return partials + ((int64_t)(c0 + k) * 2 + (k == 0 ? off : 0)) * kPart;
+  }
+};
+
+template <class T, int D, int M>
+__global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(const __grid_constant__ Attend p,
+                                                                                const __grid_constant__ CUtensorMap map) {
+  using S = Shape<T, D, M>;
+  extern __shared__ __align__(1024) char smem[];
   char* const ring = smem;
-  float* const qs = (float*)(smem + S::kStages * S::kStage);
-  int64_t* const places = (int64_t*)(qs + kWarps * S::kQuery);  // [2][kRows]
-  __shared__ uint32_t known[S::kStages + 1][S::kWords];  // which keys of a tile are tokens
-  __shared__ float ms[kWarps * M], zs[kWarps * M];       // maxima and sums that meet
-  __shared__ long long sums[kWarps];
-  __shared__ int found[3];
-  __shared__ int arrived, bad;  // bad: some table entry so far is no page
+  __shared__ Shared<T, D, M> sh;
 
   const yapd_cache& c = p.a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int shift = 31 - __clz(S::kRows / p.hg), keys = 1 << shift;  // keys of a tile
   const int pairs = p.head_groups * p.row_blocks;
+  const int group_bytes = p.hg * 16 * S::kBytes;
 
   // all units, and where this CTA's share begins
   const int per = (p.a.B + kThreads - 1) / kThreads;
@@ -663,17 +773,26 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     const long long y = __shfl_up_sync(~0u, upto, d);
     if (lane >= d) upto += y;
   }
-  if (lane == 31) sums[warp] = upto;
-  if (tid == 0) bad = 0;
+  if (lane == 31) sh.sums[warp] = upto;
+  if (tid == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      yapd::mbar_init(&sh.full[s], 33);  // the fetching warp's copies, and its word on the tile
+      yapd::mbar_init(&sh.empty[s], kWarps);
+    }
+    yapd::mbar_init(&sh.met, kWarps);
+    yapd::fence_mbar_init();
+    sh.given_up = sh.left = 0;
+  }
   __syncthreads();
   long long total = 0;
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w == warp) upto += total;
-    total += sums[w];
+    total += sh.sums[w];
   }
   const long long chunk = (total + gridDim.x - 1) / gridDim.x;
   const long long u0 = min(chunk * blockIdx.x, total), u1 = min(u0 + chunk, total);
-  if (u0 < u1 && upto - mine <= u0 && u0 < upto) {
+  const int units = (int)(u1 - u0);  // 2^31 tiles of one CTA would take it an hour
+  if (units > 0 && upto - mine <= u0 && u0 < upto) {
     long long at = upto - mine;
     for (int b = b0;; ++b) {
       int slot;
@@ -681,274 +800,384 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
       const long long n = (long long)tiles * pairs;
       if (u0 < at + n) {
         const long long r = u0 - at;
-        found[0] = b;
-        found[1] = (int)(r / tiles);
-        found[2] = (int)(r % tiles);
+        sh.found[0] = b;
+        sh.found[1] = (int)(r / tiles);
+        sh.found[2] = (int)(r % tiles);
         break;
       }
       at += n;
     }
   }
   __syncthreads();
+  constexpr int kPart = kMaxRows * (D + 2);
 
-  // requests without a token
-  for (int b = blockIdx.x; b < p.a.B; b += gridDim.x) {
-    int slot;
-    if (slot_len(p, b, slot) > 0) continue;
-    for (int x = tid; x < p.a.new_tokens * p.a.heads * (D / 4); x += kThreads) {
-      const int r = x / (D / 4), h = r % p.a.heads, i = r / p.a.heads, head = h / p.group;
-      const int row = i * p.group + h - head * p.group;
-      write_row<T>(p, b, head, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
-      if (x % (D / 4) == 0) write_lse(p, b, head, row, 0.0f, 0.0f);
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- fetch
+    // Lane y (and y + 32, ...) looks key y up: the table entry is read while the
+    // tile before it is on its way. Where pages are whole groups of 16 tokens a
+    // group's first lane copies it as two boxes; a tile with new tokens, or of
+    // other pages, goes 16 bytes a lane, token by token.
+    constexpr int kPer = S::kRows / 32;
+    constexpr int kNone = INT32_MIN;
+    constexpr int kVec = 16 / sizeof(T), kChunks = S::kBytes / 16, kIn = S::kInner / 16;
+    const int chunks = p.hg * kChunks;                      // of a token's keys
+    const int at_once = chunks >= 32 ? 1 : 32 / chunks;     // tokens of one instruction
+    const int my_token = chunks >= 32 ? 0 : lane / chunks, my_chunk = lane - my_token * chunks;
+    const bool copying = my_token < at_once;
+    const int64_t to_v = (int64_t)c.page_size * c.kv_heads * D;
+    // bytes from the stage's start to chunk x of token y's keys
+    auto chunk_at = [&](int y, int x) {
+      const int h = x / kChunks, ch = x % kChunks, tok = y & 15;
+      return (y >> 4) * group_bytes + ((ch / kIn * p.hg + h) * 16 + tok) * S::kInner + (ch % kIn << 4 ^ S::turn(tok));
+    };
+    int entry[kPer];
+    Cursor at;
+    auto ask = [&]() {
+      const int k0 = tile_start(at, shift), low = first_low(p, at.len), sinks = sinks_of(p);
+      const int32_t* const row = c.page_table + (int64_t)at.slot * c.max_pages;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int y = lane + 32 * e, j = k0 + y;
+        entry[e] = kNone;
+        if (y < keys && j < at.len && (j >= low || j < sinks)) entry[e] = max(row[div_floor(j, p.page)], -1);
+      }
+    };
+    int head0 = 0, rb = 0;
+    if (units > 0) {
+      at.b = sh.found[0];
+      at.hr = sh.found[1];
+      at.tile = sh.found[2];
+      enter(p, at, shift);
+      head0 = at.hr / p.row_blocks * p.hg;
+      rb = at.hr % p.row_blocks;
+      ask();
     }
-  }
-
-  const long long units = u1 - u0;
-  Cursor get, load, look;  // the tile that is multiplied, fetched, looked up
-  get.b = found[0];
-  get.hr = found[1];
-  get.tile = found[2];
-  if (units > 0) enter(p, get, shift);
-  load = look = get;
-
-  // Looking a tile up is two halves, so that the read of the page table is on
-  // its way during a product: thread y holds key y's table entry, then notes the
-  // token's place, in elements from the layer's start (-1: no token, -2 - i: new
-  // token i, read from the call's rows).
-  constexpr int kNone = INT32_MIN;
-  int entry;
-  auto ask = [&](const Cursor& x) {
-    const int j = tile_start(x, shift) + tid, low = first_low(p, x.len), sinks = sinks_of(p);
-    entry = kNone;
-    if (tid < keys && j < x.len && (j >= low || j < sinks))
-      entry = max(c.page_table[(int64_t)x.slot * c.max_pages + div_floor(j, p.page)], -1);
-  };
-  auto note = [&](const Cursor& x, int tile) {
-    const int j = tile_start(x, shift) + tid, i = j - (x.len - p.a.new_tokens);
-    int64_t place = -1;
-    if (entry != kNone) {
-      if (p.a.k && i >= 0) {
-        place = -2 - i;
-      } else if (entry >= 0 && entry < c.pages) {
-        const int r = j - (int)div_floor(j, p.page) * c.page_size;
-        place = entry * c.stride_page + (int64_t)r * c.kv_heads * D;
+    bool bad = false;
+    int it = 0;
+    for (int stage = 0, phase = 1; it < units; ++it) {
+      // a stage's first use needs no wait: the phase before the first counts as over
+      if (!yapd::mbar_wait_bounded(&sh.empty[stage], phase, it < S::kStages ? kWaitNs : p.wait_ns)) break;
+      const int k0 = tile_start(at, shift), fresh0 = at.len - p.a.new_tokens;
+      const bool boxes = p.boxes && (!p.a.k || k0 + keys <= fresh0);
+      const uint32_t to = smem_addr(ring + stage * S::kStage);
+      uint32_t tokens[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const bool is_new = p.a.k && k0 + lane + 32 * e >= fresh0;  // its rows are the call's
+        const bool wrong = entry[e] != kNone && !is_new && (entry[e] < 0 || entry[e] >= c.pages);
+        if (__any_sync(~0u, wrong)) {
+          bad = true;
+          if (wrong) {
+            entry[e] = kNone;
+            set_status(c.workspace, YAPD_STATUS_BAD_PAGE);
+          }
+        }
+        tokens[e] = __ballot_sync(~0u, entry[e] != kNone);
+      }
+      if (lane == 0) {
+        Tile& t = sh.tile[stage];
+        t.b = at.b;
+        t.head0 = head0;
+        t.rb = rb;
+        t.len = at.len;
+        t.k0 = k0;
+        t.tile = at.tile;
+        t.tiles = at.span.tiles;
+        // every row sees every key of the tile unless
+        const int first_end = p.a.causal ? at.len - p.a.new_tokens + 1 : at.len;
+        const int64_t last_low = p.a.window > 0 ? (int64_t)at.len - p.a.window : 0;
+        t.mixed = bad || k0 + keys > first_end || (k0 < last_low && k0 + keys > p.a.sinks);
+        t.last = at.tile + 1 == at.span.tiles || it + 1 == units;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sh.known[stage][e] = tokens[e];
+        int groups = 0;
+        if (boxes)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) groups += ((tokens[e] & 0xffffu) != 0) + (tokens[e] >> 16 != 0);
+        yapd::mbar_arrive_expect_tx(&sh.full[stage], 2 * groups * group_bytes);
+      }
+      __syncwarp();
+      if (boxes) {
+        // a group's tokens are all of one page; hidden ones come along
+        yapd::fence_proxy_async_smem();
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const uint32_t mine = lane < 16 ? tokens[e] & 0xffffu : tokens[e] & 0xffff0000u;
+          const int g = __shfl_sync(~0u, entry[e], mine ? __ffs(mine) - 1 : lane);
+          if ((lane & 15) == 0 && mine) {
+            const int y = lane + 32 * e, j = k0 + y, r = j - (int)div_floor(j, p.page) * c.page_size;
+            const uint32_t d = to + (y >> 4) * group_bytes;
+            copy_group(d, &map, &sh.full[stage], r, head0, g);
+            copy_group(d + S::kHalf, &map, &sh.full[stage], c.page_size + r, head0, g);
+          }
+        }
       } else {
-        bad = 1;
-        set_status(c.workspace, YAPD_STATUS_BAD_PAGE);
-      }
-    }
-    if (tid < S::kRows) {
-      places[(tile & 1) * S::kRows + tid] = place;
-      const uint32_t mask = __ballot_sync(~0u, place != -1);
-      if (lane == 0) known[tile & S::kStages][warp] = mask;
-    }
-  };
-  static_assert(S::kStages == 3, "a ring of four masks");
-  const int64_t to_v = (int64_t)c.page_size * c.kv_heads * D;
-  auto fetch = [&](const Cursor& x, int stage, int tile) {
-    const int head0 = x.hr / p.row_blocks * p.hg;
-    const T* const base = (const T*)c.kv + p.a.layer * c.stride_layer + head0 * D;
-    const int64_t* const at = places + (tile & 1) * S::kRows;
-    const uint32_t to = smem_addr(ring + stage * S::kStage);
-    constexpr int kVec = 16 / sizeof(T);
-    if (!p.a.k || tile_start(x, shift) + keys <= x.len - p.a.new_tokens) {
+        const T* const base = (const T*)c.kv + p.a.layer * c.stride_layer + head0 * D;
+        const int old = p.a.k ? min(fresh0 - k0, keys) : keys;  // the first ones of the tile are in the pages
 #pragma unroll
-      for (int e = 0; e < S::kLoads; ++e) {
-        const int y = tid + e * kThreads, row = y / S::kChunks, ch = y - row * S::kChunks;
-        const int64_t place = at[row & (keys - 1)];
-        const T* const k = base + max(place, (int64_t)0) + (row >> shift) * D + ch * kVec;
-        const uint32_t d = to + row * S::kPitch + ch * 16;
-        copy16(d, k, place >= 0);
-        copy16(d + S::kHalf, k + to_v, place >= 0);
-      }
-    } else {
-      for (int e = 0; e < S::kLoads; ++e) {
-        const int y = tid + e * kThreads, row = y / S::kChunks, ch = y - row * S::kChunks, h = row >> shift;
-        const int64_t place = at[row & (keys - 1)];
-        const T *k = base, *v = base;
-        if (place >= 0) {
-          k = base + place + h * D + ch * kVec;
-          v = k + to_v;
-        } else if (place < -1) {
-          const int i = (int)(-2 - place);
-          k = (const T*)p.a.k + x.b * p.a.k_stride_req + i * p.a.k_stride_pos + (head0 + h) * p.a.k_stride_head + ch * kVec;
-          v = (const T*)p.a.v + x.b * p.a.v_stride_req + i * p.a.v_stride_pos + (head0 + h) * p.a.v_stride_head + ch * kVec;
+        for (int e = 0; e < kPer; ++e) {
+          const int j = k0 + lane + 32 * e, r = j - (int)div_floor(j, p.page) * c.page_size;
+          const int64_t place = entry[e] == kNone ? -1 : entry[e] * c.stride_page + (int64_t)r * c.kv_heads * D;
+          for (int y0 = 0; y0 < 32 && y0 + 32 * e < old; y0 += at_once) {
+            const int y = 32 * e + y0 + my_token;
+            const int64_t from = __shfl_sync(~0u, place, y0 + my_token);
+            const bool read = from >= 0;
+            const T* const k = base + (read ? from : 0);
+            if (copying && y < old)
+              for (int x = my_chunk; x < chunks; x += 32) {
+                const uint32_t d = to + chunk_at(y, x);
+                copy16(d, k + x * kVec, read);
+                copy16(d + S::kHalf, k + to_v + x * kVec, read);
+              }
+          }
         }
-        const uint32_t d = to + row * S::kPitch + ch * 16;
-        copy16(d, k, place != -1);
-        copy16(d + S::kHalf, v, place != -1);
+        for (int y = max(old, 0); y < keys; ++y) {
+          const int i = k0 + y - fresh0;
+          const bool read = i < p.a.new_tokens;
+          const T* const k = (const T*)p.a.k + at.b * p.a.k_stride_req + (read ? i : 0) * p.a.k_stride_pos;
+          const T* const v = (const T*)p.a.v + at.b * p.a.v_stride_req + (read ? i : 0) * p.a.v_stride_pos;
+          for (int x = lane; x < chunks; x += 32) {
+            const int h = head0 + x / kChunks, ch = x % kChunks;
+            const uint32_t d = to + chunk_at(y, x);
+            copy16(d, k + h * p.a.k_stride_head + ch * kVec, read);
+            copy16(d + S::kHalf, v + h * p.a.v_stride_head + ch * kVec, read);
+          }
+        }
+      }
+      copies_arrive(&sh.full[stage]);
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      if (it + 1 < units) {
+        const int hr = at.hr;
+        advance(p, at, shift);
+        if (at.hr != hr) {
+          head0 = at.hr / p.row_blocks * p.hg;
+          rb = at.hr % p.row_blocks;
+        }
+        ask();
       }
     }
-  };
+    copies_wait();  // what is on its way lands before the CTA ends
+    if (it < units)
+      for (int n = max(it - S::kStages, 0); n < it; ++n)
+        yapd::mbar_wait_bounded(&sh.full[n % S::kStages], n / S::kStages & 1, kWaitNs);
+    if (it < units && lane == 0) {
+      set_status(c.workspace, YAPD_STATUS_WAIT_TIMEOUT);
+      atomicExch(&sh.given_up, 1);
+    }
+  } else {
+    // -------------------------------------------------------------- multiply
+    // requests without a token
+    for (int b = blockIdx.x; b < p.a.B; b += gridDim.x) {
+      int slot;
+      if (slot_len(p, b, slot) > 0) continue;
+      for (int x = tid; x < p.a.new_tokens * p.a.heads * (D / 4); x += kWarps * 32) {
+        const int r = x / (D / 4), h = r % p.a.heads, i = r / p.a.heads, head = h / p.group;
+        const int row = i * p.group + h - head * p.group;
+        write_row<T>(p, b, head, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
+        if (x % (D / 4) == 0) write_lse(p, b, head, row, 0.0f, 0.0f);
+      }
+    }
+    // the new tokens' rows; CTAs without a share are the last ones
+    if (p.a.k)
+      for (int x = gridDim.x - 1 - blockIdx.x; x < p.a.B * p.a.new_tokens; x += gridDim.x)
+        store_token<T>(p, x / p.a.new_tokens, x % p.a.new_tokens);
 
-  // the pipeline fills: two tiles under way, the third looked up
-  for (int s = 0; s < S::kStages; ++s) {
-    if (s < units) {
-      ask(look);
-      note(look, s);
-      advance(p, look, shift);
-    }
-    __syncthreads();
-    if (s < S::kStages - 1) {
-      if (s < units) {
-        fetch(load, s, s);
-        advance(p, load, shift);
+    const int wk_all = kWarps / p.wr, wk = warp / p.wr, wrow = warp - wk * p.wr;
+    const int parts = wk_all / p.hg;                       // warps that share a head's keys
+    const int head_in = wk / parts, part = wk - head_in * parts;
+    const int span = keys / parts;                         // keys of this warp
+    // the warp's keys: from the group's start on, and whole steps of 16 in groups of their own
+    const int mine_at = (part * span >> 4) * group_bytes + head_in * S::kSlab;
+    float* const my_qs = (float*)(smem + S::kStages * S::kStage) + warp * S::kQuery;
+    bool ok = true;
+    int meetings = 0;
+    // the multiplying warps wait for one another
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) yapd::mbar_arrive(&sh.met);
+      ok = ok && yapd::mbar_wait_bounded(&sh.met, meetings++ & 1, p.wait_ns);
+    };
+    Rows<T, D, M> w;
+    bool fresh = true, whole = true;
+    for (int it = 0, stage = 0, phase = 0; it < units; ++it) {
+      if (!(ok = yapd::mbar_wait_bounded(&sh.full[stage], phase, p.wait_ns))) break;
+      const Tile& t = sh.tile[stage];
+      const int head0 = t.head0, rb = t.rb;
+      if (fresh) {
+        whole = t.tile == 0;
+        Cursor x;
+        x.b = t.b;
+        x.len = t.len;
+        begin_rows<T, D, M>(p, w, x, head0 + head_in, (rb * p.wr + wrow) * M, my_qs);
+        fresh = false;
       }
-      copies_commit();
+      {
+        Place at;
+        at.keys = ring + stage * S::kStage + mine_at;
+        at.first = part * span & 15;
+        at.slab = p.hg * S::kSlab;
+        at.group = group_bytes;
+        const bool mixed = t.mixed;
+        const int j0 = t.k0 + part * span, len = t.len;
+        for (int x = 0; x < span; x += S::kStep) {
+          if (j0 + x >= len) break;
+          step<T, D, M, S::kStep>(p, w, at, my_qs, j0 + x, mixed, sh.known[stage], part * span + x);
+          if constexpr (S::kStep < 16) {
+            at.first += S::kStep;
+            if (at.first == 16) {
+              at.first = 0;
+              at.keys += group_bytes;
+            }
+          } else {
+            at.keys += S::kStep / 16 * group_bytes;
+          }
+        }
+      }
+      if (t.last) {
+        // the warps' triples meet in the stage that was just read
+        const bool done = t.tile + 1 == t.tiles;
+        whole = whole && done;
+        const int b = t.b;
+        const long long start = u0 + it - t.tile, end = start + t.tiles;
+        meet();
+        if (!ok) break;
+        float* const joined = (float*)(ring + stage * S::kStage);
+        put_rows<T, D, M>(w, sh.m + warp * M, sh.z + warp * M, joined + warp * M * S::kJoinPitch);
+        meet();
+        if (!ok) break;
+        const int block_rows = p.wr * M, rows_here = min(block_rows, p.rows - rb * block_rows);
+        float* const left_at = p.partials + ((int64_t)blockIdx.x * 2 + (start > u0 ? 1 : 0)) * kPart;
+        for (int x = tid; x < p.hg * rows_here * (D / 4); x += kWarps * 32) {
+          const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here, row = rr - hi * rows_here;
+          const int rm = row & (M - 1), first = (hi * parts) * p.wr + row / M;
+          float m = -INFINITY;
+          for (int k = 0; k < parts; ++k) m = fmaxf(m, sh.m[(first + k * p.wr) * M + rm]);
+          const float base = m == -INFINITY ? 0.0f : m;
+          float z = 0.0f;
+          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int k = 0; k < parts; ++k) {
+            const int y = (first + k * p.wr) * M + rm;
+            const float f = ex2(sh.m[y] - base);
+            const float4 v = *(const float4*)(joined + y * S::kJoinPitch + 4 * d);
+            z = fmaf(f, sh.z[y], z);
+            o.x = fmaf(f, v.x, o.x);
+            o.y = fmaf(f, v.y, o.y);
+            o.z = fmaf(f, v.z, o.z);
+            o.w = fmaf(f, v.w, o.w);
+          }
+          if (whole) {
+            const float rz = z == 0.0f ? 0.0f : 1.0f / z;
+            write_row<T>(p, b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
+            if (d == 0) write_lse(p, b, head0 + hi, rb * block_rows + row, m, z);
+          } else {
+            float* const to = left_at + rr * (D + 2);
+            *(float2*)(to + 4 * d) = make_float2(o.x, o.y);
+            *(float2*)(to + 4 * d + 2) = make_float2(o.z, o.w);
+            if (d == 0) *(float2*)(to + D) = make_float2(m, z);
+          }
+        }
+        yapd::fence_proxy_async_smem();  // the stage is a box's target again
+        if (!whole) {
+          const Cut cut(start, end, chunk);
+          __threadfence();
+          meet();
+          if (!ok) break;
+          if (tid == 0) {
+            sh.left |= start > u0 ? 2 : 1;
+            sh.arrived = atomicAdd(p.counters + cut.c0, 1) == cut.n - 1;
+            if (sh.arrived) p.counters[cut.c0] = 0;  // for the next call; nobody else comes
+          }
+          meet();
+          if (!ok) break;
+          if (sh.arrived) {
+            __threadfence();
+            // maxima and sums: a warp per row, lanes over the parts in their order
+            for (int rr = warp; rr < p.hg * rows_here; rr += kWarps) {
+              float m = -INFINITY, z = 0.0f;
+              for (int k = lane; k < cut.n; k += 32)
+                m = fmaxf(m, __ldcg(cut.part<kPart>(p.partials, k) + rr * (D + 2) + D));
+#pragma unroll
+              for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+              const float base = m == -INFINITY ? 0.0f : m;
+              for (int k = lane; k < cut.n; k += 32) {
+                const float2 mz = __ldcg((const float2*)(cut.part<kPart>(p.partials, k) + rr * (D + 2) + D));
+                z = fmaf(ex2(mz.x - base), mz.y, z);
+              }
+#pragma unroll
+              for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
+              if (lane == 0) {
+                const int hi = rr / rows_here;
+                sh.m[rr] = base;
+                sh.z[rr] = z == 0.0f ? 0.0f : 1.0f / z;
+                write_lse(p, b, head0 + hi, rb * block_rows + rr - hi * rows_here, m, z);
+              }
+            }
+            meet();
+            if (!ok) break;
+            for (int x = tid; x < p.hg * rows_here * (D / 2); x += kWarps * 32) {
+              const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here;
+              const float base = sh.m[rr], rz = sh.z[rr];
+              float2 o = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+              for (int k = 0; k < cut.n; ++k) {
+                const float* const y = cut.part<kPart>(p.partials, k) + rr * (D + 2);
+                const float f = ex2(__ldcg(y + D) - base);
+                const float2 v = __ldcg((const float2*)(y + 2 * d));
+                o.x = fmaf(f, v.x, o.x);
+                o.y = fmaf(f, v.y, o.y);
+              }
+              const int full = rb * block_rows + rr - hi * rows_here, i = (int)div_floor(full, p.groups);
+              const int h = (head0 + hi) * p.group + full - i * p.group;
+              T* const out = (T*)p.a.out + b * p.a.out_stride_req + i * p.a.out_stride_pos + h * p.a.out_stride_head + 2 * d;
+              if constexpr (sizeof(T) == 4)
+                *(float2*)out = make_float2(o.x * rz, o.y * rz);
+              else
+                *(uint32_t*)out = pack2<T>(o.x * rz, o.y * rz);
+            }
+          }
+        }
+        fresh = true;
+      }
+      __syncwarp();
+      if (lane == 0) yapd::mbar_arrive(&sh.empty[stage]);
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (!ok && lane == 0) {
+      set_status(c.workspace, YAPD_STATUS_WAIT_TIMEOUT);
+      atomicExch(&sh.given_up, 1);
     }
   }
-  if (p.a.k)
-    for (int x = blockIdx.x; x < p.a.B * p.a.new_tokens; x += gridDim.x)
-      store_token<T>(p, x / p.a.new_tokens, x % p.a.new_tokens);
 
-  const int wk_all = kWarps / p.wr, wk = warp / p.wr, wrow = warp - wk * p.wr;
-  const int span = S::kRows / wk_all;                    // stage rows of this warp
-  const int parts = wk_all / p.hg;                       // warps that share a head's keys
-  const int head_in = wk / parts, part = wk - head_in * parts;
-  float* const my_qs = qs + warp * S::kQuery;
-  Rows<T, D, M> w;
-  bool fresh = true, whole = true;
-  int stage = 0;
-  for (long long it = 0; it < units; ++it) {
-    copies_wait<S::kStages - 2>();
-    __syncthreads();
-    if (it + S::kStages - 1 < units) {
-      fetch(load, stage == 0 ? S::kStages - 1 : stage - 1, (int)(it + S::kStages - 1));
-      advance(p, load, shift);
-    }
-    copies_commit();
-    const bool more = it + S::kStages < units;
-    if (more) ask(look);
-    const int head0 = get.hr / p.row_blocks * p.hg, rb = get.hr % p.row_blocks;
-    if (fresh) {
-      whole = get.tile == 0;
-      begin_rows<T, D, M>(p, w, get, head0 + head_in, (rb * p.wr + wrow) * M, my_qs);
-      fresh = false;
-    }
-    {
-      const int k0 = tile_start(get, shift);
-      // every row sees every key of the tile
-      const int first_end = p.a.causal ? get.len - p.a.new_tokens + 1 : get.len;
-      const int64_t last_low = p.a.window > 0 ? (int64_t)get.len - p.a.window : 0;
-      const bool mixed = bad || k0 + keys > first_end || (k0 < last_low && k0 + keys > p.a.sinks);
-      const char* rows = ring + stage * S::kStage + wk * span * S::kPitch;
-      for (int x = 0; x < span; x += S::kStep) {
-        const int j0 = k0 + part * span + x;
-        if (j0 >= get.len) break;
-        step<T, D, M, S::kStep>(p, w, rows + x * S::kPitch, rows + S::kHalf + x * S::kPitch, my_qs, j0, mixed,
-                                known[it & S::kStages], part * span + x);
-      }
-    }
-    if (more) {
-      note(look, (int)(it + S::kStages));
-      advance(p, look, shift);
-    }
-    const bool last_tile = get.tile + 1 == get.span.tiles;
-    if (last_tile || it + 1 == units) {
-      // the warps' triples meet in the stage that was just read
-      whole = whole && last_tile;
-      __syncthreads();
-      float* const joined = (float*)(ring + stage * S::kStage);
-      put_rows<T, D, M>(w, ms + warp * M, zs + warp * M, joined + warp * M * S::kJoinPitch);
-      __syncthreads();
-      const int block_rows = p.wr * M, rows_here = min(block_rows, p.rows - rb * block_rows);
-      // which CTAs hold parts of this (request, head group, row block)
-      const long long u = u0 + it, start = u - get.tile, end = start + get.span.tiles;
-      const int c0 = (int)(start / chunk), c1 = (int)((end - 1) / chunk);
-      constexpr int64_t kPart = kMaxRows * (D + 2);
-      float* const mine_at = p.partials + ((int64_t)blockIdx.x * 2 + (start > u0 ? 1 : 0)) * kPart;
-      for (int x = tid; x < p.hg * rows_here * (D / 4); x += kThreads) {
-        const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here, row = rr - hi * rows_here;
-        const int rm = row & (M - 1), first = (hi * parts) * p.wr + row / M;
-        float m = -INFINITY;
-        for (int k = 0; k < parts; ++k) m = fmaxf(m, ms[(first + k * p.wr) * M + rm]);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float z = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < parts; ++k) {
-          const int y = (first + k * p.wr) * M + rm;
-          const float f = ex2(ms[y] - base);
-          const float4 v = *(const float4*)(joined + y * S::kJoinPitch + 4 * d);
-          z = fmaf(f, zs[y], z);
-          o.x = fmaf(f, v.x, o.x);
-          o.y = fmaf(f, v.y, o.y);
-          o.z = fmaf(f, v.z, o.z);
-          o.w = fmaf(f, v.w, o.w);
-        }
-        if (whole) {
-          const float rz = z == 0.0f ? 0.0f : 1.0f / z;
-          write_row<T>(p, get.b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
-          if (d == 0) write_lse(p, get.b, head0 + hi, rb * block_rows + row, m, z);
-        } else {
-          float* const to = mine_at + rr * (D + 2);
-          *(float2*)(to + 4 * d) = make_float2(o.x, o.y);
-          *(float2*)(to + 4 * d + 2) = make_float2(o.z, o.w);
-          if (d == 0) *(float2*)(to + D) = make_float2(m, z);
-        }
-      }
-      if (!whole) {
+  // A CTA that gave up still takes part in the counts of the pieces that it
+  // shares, with sums that are no numbers, so that the counters end at zero.
+  __syncthreads();
+  if (sh.given_up && tid == 0) {
+    Cursor x;
+    x.b = sh.found[0];
+    x.hr = sh.found[1];
+    x.tile = 0;
+    enter(p, x, shift);
+    long long start = u0 - sh.found[2];
+    while (start < u1) {
+      const long long end = start + x.span.tiles;
+      const int which = start > u0 ? 2 : 1;
+      if ((start < u0 || end > u1) && !(sh.left & which)) {
+        const Cut cut(start, end, chunk);
+        float* const to = p.partials + ((int64_t)blockIdx.x * 2 + which - 1) * kPart;
+        for (int r = 0; r < kMaxRows; ++r) *(float2*)(to + r * (D + 2) + D) = make_float2(0.0f, NAN);
         __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const int before = atomicAdd(p.counters + c0, 1);
-          arrived = before == c1 - c0;
-          if (arrived) p.counters[c0] = 0;  // for the next call; nobody else comes
-        }
-        __syncthreads();
-        if (arrived) {
-          __threadfence();
-          // the parts in their order: CTA c0's is its second unless its share begins with it
-          const int n = c1 - c0 + 1;
-          const float* const parts0 = p.partials + (c0 * 2 + (start > c0 * chunk ? 1 : 0)) * kPart;
-          const float* const parts1 = p.partials + (int64_t)c0 * 2 * kPart;
-          auto part_at = [&](int k) { return k == 0 ? parts0 : parts1 + k * 2 * kPart; };
-          // maxima and sums: a warp per row, lanes over the parts
-          for (int rr = warp; rr < p.hg * rows_here; rr += kWarps) {
-            float m = -INFINITY, z = 0.0f;
-            for (int k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(part_at(k) + rr * (D + 2) + D));
-#pragma unroll
-            for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-            const float base = m == -INFINITY ? 0.0f : m;
-            for (int k = lane; k < n; k += 32) {
-              const float2 mz = __ldcg((const float2*)(part_at(k) + rr * (D + 2) + D));
-              z = fmaf(ex2(mz.x - base), mz.y, z);
-            }
-#pragma unroll
-            for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
-            if (lane == 0) {
-              const int hi = rr / rows_here;
-              ms[rr] = base;
-              zs[rr] = z == 0.0f ? 0.0f : 1.0f / z;
-              write_lse(p, get.b, head0 + hi, rb * block_rows + rr - hi * rows_here, m, z);
-            }
-          }
-          __syncthreads();
-          for (int x = tid; x < p.hg * rows_here * (D / 2); x += kThreads) {
-            const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here;
-            const float base = ms[rr], rz = zs[rr];
-            float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-            for (int k = 0; k < n; ++k) {
-              const float* const y = part_at(k) + rr * (D + 2);
-              const float f = ex2(__ldcg(y + D) - base);
-              const float2 v = __ldcg((const float2*)(y + 2 * d));
-              o.x = fmaf(f, v.x, o.x);
-              o.y = fmaf(f, v.y, o.y);
-            }
-            const int full = rb * block_rows + rr - hi * rows_here, i = (int)div_floor(full, p.groups);
-            const int h = (head0 + hi) * p.group + full - i * p.group;
-            T* const out = (T*)p.a.out + get.b * p.a.out_stride_req + i * p.a.out_stride_pos + h * p.a.out_stride_head + 2 * d;
-            if constexpr (sizeof(T) == 4)
-              *(float2*)out = make_float2(o.x * rz, o.y * rz);
-            else
-              *(uint32_t*)out = pack(from_f32<T>(o.x * rz), from_f32<T>(o.y * rz));
-          }
-        }
+        if (atomicAdd(p.counters + cut.c0, 1) == cut.n - 1) p.counters[cut.c0] = 0;
       }
-      fresh = true;
+      start = end;
+      x.tile = x.span.tiles - 1;
+      advance(p, x, shift);
     }
-    advance(p, get, shift);
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
   }
 }
 
@@ -973,6 +1202,45 @@ int grid_of(int& grid) {
   return YAPD_OK;
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static std::once_flag once;
+  static EncodeTiledFn fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(f);
+  });
+  return fn;
+}
+
+// The layer's pages as (row of a slab, token of both halves, head, slab of a
+// head, page); a box is 16 tokens of the unit's heads.
+template <class T, int D, int M>
+bool encode(const Attend& p, CUtensorMap& map) {
+  using S = Shape<T, D, M>;
+  const EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const yapd_cache& c = p.a.cache;
+  const cuuint32_t inner = S::kInner / sizeof(T);
+  const int64_t block = (int64_t)2 * c.page_size * c.kv_heads * D;
+  const cuuint64_t dims[5] = {inner, (cuuint64_t)2 * c.page_size, (cuuint64_t)c.kv_heads, S::kSlabs, (cuuint64_t)c.pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)c.kv_heads * S::kBytes, S::kBytes, S::kInner,
+                                 (cuuint64_t)(c.pages > 1 ? c.stride_page : block) * sizeof(T)};
+  const cuuint32_t box[5] = {inner, 16, (cuuint32_t)p.hg, S::kSlabs, 1}, step[5] = {1, 1, 1, 1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : p.a.cache.dtype == YAPD_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return fn(&map, type, 5, (T*)c.kv + p.a.layer * c.stride_layer, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            S::kInner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class T, int D, int M>
 int launch(Attend& p, cudaStream_t st) {
   int grid = 0;
@@ -984,10 +1252,13 @@ int launch(Attend& p, cudaStream_t st) {
   // in its page.  Few requests are shared out by heads first, so that fewer
   // CTAs hold parts of the same sums.
   const int kvh = p.a.cache.kv_heads;
-  p.hg = 4 / p.wr;
+  p.hg = Shape<T, D, M>::kMaxHeads >= p.wr ? Shape<T, D, M>::kMaxHeads / p.wr : 1;
   while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < grid / 2)) p.hg /= 2;
   p.head_groups = kvh / p.hg;
-  attend_kernel<T, D, M><<<grid, kThreads, Shape<T, D, M>::kSmem, st>>>(p);
+  CUtensorMap map{};
+  p.boxes = p.a.cache.page_size % 16 == 0;
+  if (p.boxes && !encode<T, D, M>(p, map)) return YAPD_ERR_LAUNCH;
+  attend_kernel<T, D, M><<<grid, kThreads, Shape<T, D, M>::kSmem, st>>>(p, map);
   return launched();
 }
 
@@ -1050,6 +1321,7 @@ extern "C" int yapd_attend(const yapd_attend_args* args, void* stream) {
   // a negative scale is a positive one of the negative queries
   p.negate = std::signbit(a.scale) ? dt == YAPD_DTYPE_F32 ? 0x80000000u : 0x80008000u : 0u;
   p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
+  p.wait_ns = a.wait_limit_ns ? a.wait_limit_ns : kWaitNs;
   char* const scratch = (char*)a.cache.workspace + kHeaderBytes + pages_scratch_bytes(a.cache);
   p.counters = (int*)scratch;
   p.partials = (float*)(scratch + round_up(kMaxCtas * 4, 256));

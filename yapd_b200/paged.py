@@ -108,7 +108,8 @@ class PagedCache:
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None, *,
                slots: torch.Tensor | None = None, causal: bool = True, window: int = 0, sinks: int = 0,
-               scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+               scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
+               wait_limit_ns: int = 0):
         """Attention of each request's last tokens over its pages in ``layer``.
 
         ``q`` is ``(B, heads, D)`` for one new token per request or ``(B, T,
@@ -124,7 +125,8 @@ class PagedCache:
         if not given.  A query that sees nothing gets zeros (and an ``lse`` of
         -inf).  Returns the output in ``q``'s shape and type, with
         ``return_lse`` also the ``(B, T, heads)`` or ``(B, heads)`` float32
-        logarithms of the softmax's sums.
+        logarithms of the softmax's sums.  ``wait_limit_ns`` bounds each wait for
+        a copy, as in ``select_step``.
         """
         a, kv = self._attend, self.kv
         shape = q.shape
@@ -178,7 +180,7 @@ class PagedCache:
         lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
         a.lse = lse.data_ptr() if return_lse else None
         a.scale = D ** -0.5 if scale is None else scale
-        a.causal, a.window, a.sinks = 1 if causal else 0, window, sinks
+        a.causal, a.window, a.sinks, a.wait_limit_ns = 1 if causal else 0, window, sinks, wait_limit_ns
         self._call(self._lib.yapd_attend, a)
         return (out, lse) if return_lse else out
 
