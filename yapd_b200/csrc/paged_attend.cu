@@ -28,6 +28,7 @@ constexpr int kWarps = 4;                     // that multiply; one more fetches
 constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kMaxRows = 64;  // query rows times key heads of a unit at most
 constexpr int64_t kWaitNs = 500000000;
+constexpr int kJoin = 4;
 
 struct Attend {
   yapd_attend_args a;
@@ -67,14 +68,13 @@ struct Shape {
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kStages = 3;
   static constexpr int kMaxHeads = kRows / 16 < kWarps ? kRows / 16 : kWarps;  // key heads of a tile
-  static constexpr int kJoinPitch = D;               // floats
   static constexpr int kWords = kRows / 32;          // of a mask of a tile's keys
   static constexpr int kQuery = sizeof(T) == 4 ? M * (D + 4) : 0;  // floats of a warp's queries in shared memory
   static constexpr int kSmem = kStages * kStage + kWarps * kQuery * 4;
   // CTAs of an SM: as many as its 228 KB hold, and no more than leave a thread the registers of its sums
   static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 1024), kMost = M == 16 ? 3 : 4;
   static constexpr int kFit = kRoom < kMost ? kRoom : kMost;
-  static_assert(kWarps * M * kJoinPitch * 4 <= kStage, "the warps' triples meet in a stage");
+  static_assert(kWarps * M * D * 4 <= kStage, "the warps' triples meet in a stage");
 
   // Where 16-byte chunk `ch` of a row lies: token `tok` (of 16).
   __device__ static __forceinline__ int turn(int tok) { return (kInner == 128 ? tok & 7 : tok >> 1 & 3) << 4; }
@@ -143,9 +143,8 @@ __device__ __forceinline__ int tile_start(const Cursor& c, int shift) {
 
 __device__ __forceinline__ uint32_t smem_addr(const void* x) { return (uint32_t)__cvta_generic_to_shared(x); }
 
-// 16 bytes to shared memory, or zeros where `from` is not to be read.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(read ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 // A box of 16 tokens of one page, all slabs of the unit's heads.
 __device__ __forceinline__ void copy_group(uint32_t to, const CUtensorMap* map, uint64_t* bar, int token, int head, int page) {
@@ -617,11 +616,14 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Pl
   values<T, D, M, N, false>(w.o, s, at);
 }
 
+// Where the sums of a row's dim `d` meet: rows that are stored together lie in different banks.
+template <int D>
+__device__ __forceinline__ int meet_at(int row, int d) { return row * D + (d ^ ((row ^ row >> 2) & 3) << 3); }
+
 // A warp's triples to shared memory: maxima and sums by row, o by (row, dim).
 template <class T, int D, int M>
 __device__ __forceinline__ void put_rows(Rows<T, D, M>& w, float* ms, float* zs, float* joined) {
   using R = Rows<T, D, M>;
-  constexpr int kJoin = Shape<T, D, M>::kJoinPitch;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int r = 0; r < R::kOwn; ++r) {
@@ -638,22 +640,27 @@ __device__ __forceinline__ void put_rows(Rows<T, D, M>& w, float* ms, float* zs,
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if constexpr (M == 4) w.o[d][e] += __shfl_xor_sync(~0u, w.o[d][e], 2);
-        if (2 * t < M) joined[(2 * t + (e & 1)) * kJoin + 16 * d + g + 8 * (e >> 1)] = w.o[d][e];
+        if (2 * t < M) joined[meet_at<D>(2 * t + (e & 1), 16 * d + g + 8 * (e >> 1))] = w.o[d][e];
       }
     } else {
 #pragma unroll
       for (int r = 0; r < R::kOwn; ++r)
-        if (g < M) *(float2*)(joined + (g + 8 * r) * kJoin + 8 * d + 2 * t) = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
+        if (g < M) *(float2*)(joined + meet_at<D>(g + 8 * r, 8 * d + 2 * t)) = make_float2(w.o[d][2 * r], w.o[d][2 * r + 1]);
     }
   }
 }
 
 // ----------------------------------------------------------------- the kernel
 
-// Stores one new token's rows (all heads) in its page.
+// The new tokens' rows to their pages: a warp per (request, token). The
+// attention that reads them waits for this kernel on the device.
 template <class T>
-__device__ void store_token(const Attend& p, int b, int i) {
+__global__ void __launch_bounds__(128) store_kernel(const __grid_constant__ Attend p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const yapd_cache& c = p.a.cache;
+  const int lane = threadIdx.x & 31, x = blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (x >= p.a.B * p.a.new_tokens) return;
+  const int b = x / p.a.new_tokens, i = x - b * p.a.new_tokens;
   int slot;
   const int t = slot_len(p, b, slot) - p.a.new_tokens + i;
   uint32_t wrong = 0;
@@ -671,19 +678,22 @@ __device__ void store_token(const Attend& p, int b, int i) {
       wrong = YAPD_STATUS_SHARED_PAGE;
   }
   if (wrong) {
-    if (threadIdx.x == 0) set_status(c.workspace, wrong);
+    if (lane == 0) set_status(c.workspace, wrong);
     return;
   }
   constexpr int kVec = 16 / sizeof(T);
   const int per = c.head_dim / kVec, all = c.kv_heads * per;
-  T* to = (T*)c.kv + p.a.layer * c.stride_layer + g * c.stride_page + (int64_t)(t - q * c.page_size) * c.kv_heads * c.head_dim;
-  T* to_v = to + (int64_t)c.page_size * c.kv_heads * c.head_dim;
-  for (int x = threadIdx.x; x < all; x += kWarps * 32) {
-    const int h = x / per, d = (x - h * per) * kVec;
-    const uint4 k = *(const uint4*)((const T*)p.a.k + b * p.a.k_stride_req + i * p.a.k_stride_pos + h * p.a.k_stride_head + d);
-    const uint4 v = *(const uint4*)((const T*)p.a.v + b * p.a.v_stride_req + i * p.a.v_stride_pos + h * p.a.v_stride_head + d);
-    *(uint4*)(to + (int64_t)x * kVec) = k;
-    *(uint4*)(to_v + (int64_t)x * kVec) = v;
+  T* const to = (T*)c.kv + p.a.layer * c.stride_layer + g * c.stride_page +
+                (int64_t)(t - q * c.page_size) * c.kv_heads * c.head_dim;
+  T* const to_v = to + (int64_t)c.page_size * c.kv_heads * c.head_dim;
+  const T* const k = (const T*)p.a.k + b * p.a.k_stride_req + i * p.a.k_stride_pos;
+  const T* const v = (const T*)p.a.v + b * p.a.v_stride_req + i * p.a.v_stride_pos;
+#pragma unroll 4
+  for (int y = lane; y < all; y += 32) {
+    const int h = y / per, d = (y - h * per) * kVec;
+    const uint4 kx = *(const uint4*)(k + h * p.a.k_stride_head + d), vx = *(const uint4*)(v + h * p.a.v_stride_head + d);
+    *(uint4*)(to + (int64_t)y * kVec) = kx;
+    *(uint4*)(to_v + (int64_t)y * kVec) = vx;
   }
 }
 
@@ -753,6 +763,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
 
   const yapd_cache& c = p.a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (p.boxes && tid == kWarps * 32) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
   const int shift = 31 - __clz(S::kRows / p.hg), keys = 1 << shift;  // keys of a tile
   const int pairs = p.head_groups * p.row_blocks;
   const int group_bytes = p.hg * 16 * S::kBytes;
@@ -815,8 +826,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     // ---------------------------------------------------------------- fetch
     // Lane y (and y + 32, ...) looks key y up: the table entry is read while the
     // tile before it is on its way. Where pages are whole groups of 16 tokens a
-    // group's first lane copies it as two boxes; a tile with new tokens, or of
-    // other pages, goes 16 bytes a lane, token by token.
+    // group's first lane copies it as two boxes; of other pages the warp copies
+    // token by token, 16 bytes a lane.
     constexpr int kPer = S::kRows / 32;
     constexpr int kNone = INT32_MIN;
     constexpr int kVec = 16 / sizeof(T), kChunks = S::kBytes / 16, kIn = S::kInner / 16;
@@ -852,19 +863,20 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
       rb = at.hr % p.row_blocks;
       ask();
     }
+    // the pages are read from here on
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("fence.proxy.async;" ::: "memory");
     bool bad = false;
     int it = 0;
     for (int stage = 0, phase = 1; it < units; ++it) {
       // a stage's first use needs no wait: the phase before the first counts as over
       if (!yapd::mbar_wait_bounded(&sh.empty[stage], phase, it < S::kStages ? kWaitNs : p.wait_ns)) break;
-      const int k0 = tile_start(at, shift), fresh0 = at.len - p.a.new_tokens;
-      const bool boxes = p.boxes && (!p.a.k || k0 + keys <= fresh0);
+      const int k0 = tile_start(at, shift);
       const uint32_t to = smem_addr(ring + stage * S::kStage);
       uint32_t tokens[kPer];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        const bool is_new = p.a.k && k0 + lane + 32 * e >= fresh0;  // its rows are the call's
-        const bool wrong = entry[e] != kNone && !is_new && (entry[e] < 0 || entry[e] >= c.pages);
+        const bool wrong = entry[e] != kNone && (entry[e] < 0 || entry[e] >= c.pages);
         if (__any_sync(~0u, wrong)) {
           bad = true;
           if (wrong) {
@@ -891,13 +903,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
 #pragma unroll
         for (int e = 0; e < kPer; ++e) sh.known[stage][e] = tokens[e];
         int groups = 0;
-        if (boxes)
+        if (p.boxes)
 #pragma unroll
           for (int e = 0; e < kPer; ++e) groups += ((tokens[e] & 0xffffu) != 0) + (tokens[e] >> 16 != 0);
         yapd::mbar_arrive_expect_tx(&sh.full[stage], 2 * groups * group_bytes);
       }
       __syncwarp();
-      if (boxes) {
+      if (p.boxes) {
         // a group's tokens are all of one page; hidden ones come along
         yapd::fence_proxy_async_smem();
 #pragma unroll
@@ -913,34 +925,20 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         }
       } else {
         const T* const base = (const T*)c.kv + p.a.layer * c.stride_layer + head0 * D;
-        const int old = p.a.k ? min(fresh0 - k0, keys) : keys;  // the first ones of the tile are in the pages
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
           const int j = k0 + lane + 32 * e, r = j - (int)div_floor(j, p.page) * c.page_size;
           const int64_t place = entry[e] == kNone ? -1 : entry[e] * c.stride_page + (int64_t)r * c.kv_heads * D;
-          for (int y0 = 0; y0 < 32 && y0 + 32 * e < old; y0 += at_once) {
+          for (int y0 = 0; y0 < 32 && y0 + 32 * e < keys; y0 += at_once) {
             const int y = 32 * e + y0 + my_token;
             const int64_t from = __shfl_sync(~0u, place, y0 + my_token);
-            const bool read = from >= 0;
-            const T* const k = base + (read ? from : 0);
-            if (copying && y < old)
+            const T* const k = base + from;
+            if (copying && from >= 0)
               for (int x = my_chunk; x < chunks; x += 32) {
                 const uint32_t d = to + chunk_at(y, x);
-                copy16(d, k + x * kVec, read);
-                copy16(d + S::kHalf, k + to_v + x * kVec, read);
+                copy16(d, k + x * kVec);
+                copy16(d + S::kHalf, k + to_v + x * kVec);
               }
-          }
-        }
-        for (int y = max(old, 0); y < keys; ++y) {
-          const int i = k0 + y - fresh0;
-          const bool read = i < p.a.new_tokens;
-          const T* const k = (const T*)p.a.k + at.b * p.a.k_stride_req + (read ? i : 0) * p.a.k_stride_pos;
-          const T* const v = (const T*)p.a.v + at.b * p.a.v_stride_req + (read ? i : 0) * p.a.v_stride_pos;
-          for (int x = lane; x < chunks; x += 32) {
-            const int h = head0 + x / kChunks, ch = x % kChunks;
-            const uint32_t d = to + chunk_at(y, x);
-            copy16(d, k + h * p.a.k_stride_head + ch * kVec, read);
-            copy16(d + S::kHalf, v + h * p.a.v_stride_head + ch * kVec, read);
           }
         }
       }
@@ -980,11 +978,6 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         if (x % (D / 4) == 0) write_lse(p, b, head, row, 0.0f, 0.0f);
       }
     }
-    // the new tokens' rows; CTAs without a share are the last ones
-    if (p.a.k)
-      for (int x = gridDim.x - 1 - blockIdx.x; x < p.a.B * p.a.new_tokens; x += gridDim.x)
-        store_token<T>(p, x / p.a.new_tokens, x % p.a.new_tokens);
-
     const int wk_all = kWarps / p.wr, wk = warp / p.wr, wrow = warp - wk * p.wr;
     const int parts = wk_all / p.hg;                       // warps that share a head's keys
     const int head_in = wk / parts, part = wk - head_in * parts;
@@ -1045,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         meet();
         if (!ok) break;
         float* const joined = (float*)(ring + stage * S::kStage);
-        put_rows<T, D, M>(w, sh.m + warp * M, sh.z + warp * M, joined + warp * M * S::kJoinPitch);
+        put_rows<T, D, M>(w, sh.m + warp * M, sh.z + warp * M, joined + warp * M * D);
         meet();
         if (!ok) break;
         const int block_rows = p.wr * M, rows_here = min(block_rows, p.rows - rb * block_rows);
@@ -1061,7 +1054,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
           for (int k = 0; k < parts; ++k) {
             const int y = (first + k * p.wr) * M + rm;
             const float f = ex2(sh.m[y] - base);
-            const float4 v = *(const float4*)(joined + y * S::kJoinPitch + 4 * d);
+            const float4 v = *(const float4*)(joined + y / M * M * D + meet_at<D>(rm, 4 * d));
             z = fmaf(f, sh.z[y], z);
             o.x = fmaf(f, v.x, o.x);
             o.y = fmaf(f, v.y, o.y);
@@ -1094,41 +1087,37 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
           if (!ok) break;
           if (sh.arrived) {
             __threadfence();
-            // maxima and sums: a warp per row, lanes over the parts in their order
-            for (int rr = warp; rr < p.hg * rows_here; rr += kWarps) {
-              float m = -INFINITY, z = 0.0f;
-              for (int k = lane; k < cut.n; k += 32)
-                m = fmaxf(m, __ldcg(cut.part<kPart>(p.partials, k) + rr * (D + 2) + D));
-#pragma unroll
-              for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-              const float base = m == -INFINITY ? 0.0f : m;
-              for (int k = lane; k < cut.n; k += 32) {
-                const float2 mz = __ldcg((const float2*)(cut.part<kPart>(p.partials, k) + rr * (D + 2) + D));
-                z = fmaf(ex2(mz.x - base), mz.y, z);
-              }
-#pragma unroll
-              for (int d = 16; d; d >>= 1) z += __shfl_xor_sync(~0u, z, d);
-              if (lane == 0) {
-                const int hi = rr / rows_here;
-                sh.m[rr] = base;
-                sh.z[rr] = z == 0.0f ? 0.0f : 1.0f / z;
-                write_lse(p, b, head0 + hi, rb * block_rows + rr - hi * rows_here, m, z);
-              }
-            }
-            meet();
-            if (!ok) break;
+            // four parts at a time, in their order: their reads go out together
             for (int x = tid; x < p.hg * rows_here * (D / 2); x += kWarps * 32) {
               const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here;
-              const float base = sh.m[rr], rz = sh.z[rr];
+              float m = -INFINITY, z = 0.0f;
               float2 o = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-              for (int k = 0; k < cut.n; ++k) {
-                const float* const y = cut.part<kPart>(p.partials, k) + rr * (D + 2);
-                const float f = ex2(__ldcg(y + D) - base);
-                const float2 v = __ldcg((const float2*)(y + 2 * d));
-                o.x = fmaf(f, v.x, o.x);
-                o.y = fmaf(f, v.y, o.y);
+              for (int k0 = 0; k0 < cut.n; k0 += kJoin) {
+                float2 mz[kJoin], v[kJoin];
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k) {
+                  const float* const y = cut.part<kPart>(p.partials, min(k0 + k, cut.n - 1)) + rr * (D + 2);
+                  mz[k] = __ldcg((const float2*)(y + D));
+                  v[k] = __ldcg((const float2*)(y + 2 * d));
+                }
+                float top = m;
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k) top = fmaxf(top, mz[k].x);
+                const float base = top == -INFINITY ? 0.0f : top, f0 = ex2(m - base);
+                z *= f0;
+                o.x *= f0;
+                o.y *= f0;
+#pragma unroll
+                for (int k = 0; k < kJoin; ++k)
+                  if (k0 + k < cut.n) {
+                    const float f = ex2(mz[k].x - base);
+                    z = fmaf(f, mz[k].y, z);
+                    o.x = fmaf(f, v[k].x, o.x);
+                    o.y = fmaf(f, v[k].y, o.y);
+                  }
+                m = top;
               }
+              const float rz = z == 0.0f ? 0.0f : 1.0f / z;
               const int full = rb * block_rows + rr - hi * rows_here, i = (int)div_floor(full, p.groups);
               const int h = (head0 + hi) * p.group + full - i * p.group;
               T* const out = (T*)p.a.out + b * p.a.out_stride_req + i * p.a.out_stride_pos + h * p.a.out_stride_head + 2 * d;
@@ -1136,6 +1125,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
                 *(float2*)out = make_float2(o.x * rz, o.y * rz);
               else
                 *(uint32_t*)out = pack2<T>(o.x * rz, o.y * rz);
+              if (d == 0) write_lse(p, b, head0 + hi, full, m, z);
             }
           }
         }
@@ -1258,7 +1248,22 @@ int launch(Attend& p, cudaStream_t st) {
   CUtensorMap map{};
   p.boxes = p.a.cache.page_size % 16 == 0;
   if (p.boxes && !encode<T, D, M>(p, map)) return YAPD_ERR_LAUNCH;
-  attend_kernel<T, D, M><<<grid, kThreads, Shape<T, D, M>::kSmem, st>>>(p, map);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Shape<T, D, M>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute early{};
+  if (p.a.k) {
+    const int rows = p.a.B * p.a.new_tokens;
+    store_kernel<T><<<(rows + 3) / 4, 128, 0, st>>>(p);
+    // the attention's CTAs start beside the stores and wait for them where they read the pages
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+  }
+  if (cudaLaunchKernelEx(&cfg, attend_kernel<T, D, M>, p, map) != cudaSuccess) return YAPD_ERR_LAUNCH;
   return launched();
 }
 
