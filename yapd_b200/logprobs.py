@@ -46,30 +46,31 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     R, V = logits.shape
     if (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
-    dev = logits.device
+    dev, index = logits.device, logits.get_device()
     a = N.LogprobsArgs()
     a.R, a.V, a.top_n, a.logits_dtype = R, V, top_n, _DTYPES[logits.dtype]
     a.logits, a.stride_row = logits.data_ptr(), logits.stride(0)
-    values = torch.empty(2 + top_n, R, dtype=torch.float32, device=dev)
     logprob = top = ids = None
     if targets is not None:
-        if tuple(targets.shape) != (R,) or targets.dtype not in (torch.int64, torch.int32) or targets.device != dev:
+        if targets.shape != (R,) or targets.dtype not in (torch.int64, torch.int32) or targets.get_device() != index:
             raise ValueError(f"targets must be an int64 or int32 ({R},) tensor on {dev}")
-        targets = targets.to(torch.int64).contiguous()
-        a.targets = targets.data_ptr()
-        logprob = values[0]
-        a.logprob = logprob.data_ptr()
-    entropy = values[1]
+        if targets.dtype != torch.int64 or not targets.is_contiguous():
+            targets = targets.to(torch.int64).contiguous()
+        logprob = torch.empty(R, dtype=torch.float32, device=dev)
+        a.targets, a.logprob = targets.data_ptr(), logprob.data_ptr()
+    entropy = torch.empty(R, dtype=torch.float32, device=dev)
     a.entropy = entropy.data_ptr()
     if top_n:
-        top = values[2:].view(R, top_n)
+        top = torch.empty(R, top_n, dtype=torch.float32, device=dev)
         ids = torch.empty(R, top_n, dtype=torch.int32, device=dev)
         a.top_logprobs, a.top_ids = top.data_ptr(), ids.data_ptr()
     if R:
-        if torch.cuda.current_device() == dev.index:
-            rc = N.lib().yapd_token_logprobs(a, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
+        entry = N.lib().yapd_token_logprobs
+        if torch.cuda.current_device() == index:
+            rc = entry(a, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(dev):
-                rc = N.lib().yapd_token_logprobs(a, C.c_void_p(torch.cuda.current_stream(dev).cuda_stream))
-        N.check(rc)
+                rc = entry(a, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            N.check(rc)
     return TokenLogprobs(logprob, entropy, top, ids)

@@ -33,14 +33,6 @@ from . import _native as N
 _DTYPES = {torch.float32: N.YAPD_DTYPE_F32, torch.bfloat16: N.YAPD_DTYPE_BF16, torch.float16: N.YAPD_DTYPE_F16}
 
 
-def _rows(t: torch.Tensor, vec: int) -> torch.Tensor:
-    """``t`` itself if the kernels can read its rows of the last dimension, else a contiguous copy."""
-    st = t.stride()
-    if st[-1] != 1 or t.data_ptr() % 16 or any(s % vec for s in st[:-1]):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
 class PagedCache:
     """Pages ``kv`` ``(layers, pages, 2, page_size, kv_heads, head_dim)`` in
     float32, bfloat16 or float16, with the tables of ``slots`` requests.
@@ -76,7 +68,8 @@ class PagedCache:
         self.kv, self.page_table, self.kv_len, self.refs = kv, page_table, kv_len, refs
         self.slots, self.device = slots, dev
         self._vec = 16 // kv.element_size()
-        self._heads, self._dim = kv.shape[4], kv.shape[5]
+        self._layers, self._heads, self._dim, self._dtype, self._index = layers, kv.shape[4], kv.shape[5], kv.dtype, \
+            kv.get_device()
         c = N.Cache()
         c.layers, c.pages, _, c.page_size, c.kv_heads, c.head_dim = kv.shape
         c.dtype, c.slots, c.max_pages = _DTYPES[kv.dtype], slots, page_table.shape[1]
@@ -128,33 +121,35 @@ class PagedCache:
         logarithms of the softmax's sums.  ``wait_limit_ns`` bounds each wait for
         a copy, as in ``select_step``.
         """
-        a, kv = self._attend, self.kv
+        a, dtype, index = self._attend, self._dtype, self._index
         shape = q.shape
-        if q.dim() == 3:
+        if len(shape) == 3:
             q = q.unsqueeze(1)
             k = k if k is None or k.dim() != 3 else k.unsqueeze(1)
             v = v if v is None or v.dim() != 3 else v.unsqueeze(1)
-        if q.dim() != 4 or q.shape[3] != self._dim or q.shape[2] % self._heads or q.shape[2] == 0:
+        if q.dim() != 4:
+            raise ValueError(f"q must be (B, [T,] heads, {self._dim}), got {tuple(shape)}")
+        B, T, H, D = q.shape
+        if D != self._dim or H % self._heads or H == 0:
             raise ValueError(f"q must be (B, [T,] heads, {self._dim}) with heads a multiple of {self._heads}, "
                              f"got {tuple(shape)}")
-        B, T, H, D = q.shape
         if not 1 <= T <= N.YAPD_MAX_NEW_TOKENS:
             raise ValueError(f"1 to {N.YAPD_MAX_NEW_TOKENS} new tokens, got {T}")
-        if q.dtype != kv.dtype or q.device != kv.device:
-            raise TypeError(f"q must be {kv.dtype} on {kv.device}")
-        if not 0 <= layer < kv.shape[0]:
-            raise ValueError(f"layer {layer} of {kv.shape[0]}")
+        if q.dtype != dtype or q.get_device() != index:
+            raise TypeError(f"q must be {dtype} on {self.device}")
+        if not 0 <= layer < self._layers:
+            raise ValueError(f"layer {layer} of {self._layers}")
         if sinks < 0:
             raise ValueError("sinks must not be negative")
         if slots is not None:
             self._check_list("slots", slots, B)
+            a.slots = slots.data_ptr()
         elif B > self.slots:
             raise ValueError(f"{B} requests, but {self.slots} slots")
-        q = _rows(q, self._vec)
-        a.layer, a.B, a.new_tokens, a.heads = layer, B, T, H
-        a.slots = None if slots is None else slots.data_ptr()
-        a.q = q.data_ptr()
-        a.q_stride_req, a.q_stride_pos, a.q_stride_head, _ = q.stride()
+        else:
+            a.slots = None
+        q, (a.q_stride_req, a.q_stride_pos, a.q_stride_head, _) = self._rows(q)
+        a.layer, a.B, a.new_tokens, a.heads, a.q = layer, B, T, H, q.data_ptr()
         if k is None and v is None:
             a.k = a.v = None
         else:
@@ -163,21 +158,20 @@ class PagedCache:
             want = (B, T, self._heads, D)
             if k.shape != want or v.shape != want:
                 raise ValueError(f"k and v must be {want}, got {tuple(k.shape)} and {tuple(v.shape)}")
-            if k.dtype != kv.dtype or v.dtype != kv.dtype or k.device != kv.device or v.device != kv.device:
-                raise TypeError(f"k and v must be {kv.dtype} on {kv.device}")
-            k, v = _rows(k, self._vec), _rows(v, self._vec)
+            if k.dtype != dtype or v.dtype != dtype or k.get_device() != index or v.get_device() != index:
+                raise TypeError(f"k and v must be {dtype} on {self.device}")
+            k, (a.k_stride_req, a.k_stride_pos, a.k_stride_head, _) = self._rows(k)
+            v, (a.v_stride_req, a.v_stride_pos, a.v_stride_head, _) = self._rows(v)
             a.k, a.v = k.data_ptr(), v.data_ptr()
-            a.k_stride_req, a.k_stride_pos, a.k_stride_head, _ = k.stride()
-            a.v_stride_req, a.v_stride_pos, a.v_stride_head, _ = v.stride()
         if out is None:
-            out = torch.empty(shape, dtype=q.dtype, device=q.device)
-        elif out.shape != shape or out.dtype != q.dtype or out.device != q.device or \
-                _rows(out, self._vec) is not out:
-            raise ValueError(f"out must be a {tuple(shape)} {q.dtype} tensor on {q.device} whose rows are aligned")
-        o = out.unsqueeze(1) if out.dim() == 3 else out
+            out = torch.empty(shape, dtype=dtype, device=self.device) if len(shape) == 3 or not q.is_contiguous() \
+                else torch.empty_like(q)
+        elif out.shape != shape or out.dtype != dtype or out.get_device() != index or self._rows(out)[0] is not out:
+            raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor on {self.device} whose rows are aligned")
         a.out = out.data_ptr()
-        a.out_stride_req, a.out_stride_pos, a.out_stride_head, _ = o.stride()
-        lse = torch.empty(shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        st = out.stride()
+        a.out_stride_req, a.out_stride_pos, a.out_stride_head = st[:3] if len(st) == 4 else (st[0], 0, st[1])
+        lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
         a.lse = lse.data_ptr() if return_lse else None
         a.scale = D ** -0.5 if scale is None else scale
         a.causal, a.window, a.sinks, a.wait_limit_ns = 1 if causal else 0, window, sinks, wait_limit_ns
@@ -264,11 +258,21 @@ class PagedCache:
 
     # --------------------------------------------------------------- private
 
-    def _stream(self) -> C.c_void_p:
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+    def _rows(self, t: torch.Tensor):
+        """``t`` and its strides if the kernels can read its rows of the last
+        dimension, else those of a contiguous copy."""
+        st = t.stride()
+        vec = self._vec
+        if st[-1] != 1 or t.data_ptr() % 16 or st[0] % vec or st[1] % vec or st[-2] % vec:
+            t = t.clone(memory_format=torch.contiguous_format)
+            st = t.stride()
+        return t, st
+
+    def _stream(self) -> int:
+        return torch._C._cuda_getCurrentRawStream(self._index)
 
     def _call(self, entry, args) -> None:
-        if torch.cuda.current_device() == self.device.index:
+        if torch.cuda.current_device() == self._index:
             rc = entry(args, self._stream())
         else:
             with torch.cuda.device(self.device):
@@ -277,7 +281,7 @@ class PagedCache:
             N.check(rc)
 
     def _check_list(self, name: str, t: torch.Tensor, n: int) -> None:
-        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != self.device or \
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != self._index or \
                 (n > 1 and t.stride(0) != 1):
             raise ValueError(f"{name} must be a contiguous int32 ({n},) tensor on {self.device}")
 
