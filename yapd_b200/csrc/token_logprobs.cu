@@ -3,14 +3,15 @@
 // With m the largest logit, z = sum e^(x - m) and w = sum e^(x - m) (x - m):
 // log p(t) = x_t - m - ln z and the entropy is ln z - w / z, which has no
 // cancellation where one token has nearly all the mass. The alternatives need
-// no sort of the row: of the maxima of 64 disjoint parts of it, the n-th largest
+// no sort of the row: of the maxima of 32 disjoint parts of it, the n-th largest
 // has n tokens at or above it, so only tokens that reach it can be among the
-// first n. About 1.2 n do in a row without structure; they are listed and
-// ranked against one another.
+// first n. In a row without structure -32 ln(1 - n / 32) do, 9 for n = 8, 31 for
+// n = 20; they are listed and sorted.
 //
-// A row is held in the registers of one CTA, or of a cluster of up to eight that
-// meet in the first one's shared memory, so it is read once; a row too long for
-// that is read a second time, out of L2.
+// A warp holds up to 1056 vectors of 16 bytes in its registers and makes all
+// passes over them alone; the parts are its lanes. A longer row, or few rows,
+// are shared out over the warps of a CTA or of a cluster; a part is then the
+// same lane of a CTA's warps, and the CTAs' tokens are merged at the end.
 #include <cooperative_groups.h>
 
 #include "select_common.cuh"
@@ -21,17 +22,22 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
-constexpr int kVecs = 8;         // 16-byte vectors of a thread at a time
-constexpr int kBuckets = kThreads / 4;
-constexpr int kList = 512;       // tokens that can be ranked at once
-constexpr int kMaxCluster = 8;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kFit = 3;             // CTAs of an SM: 168 registers a thread
+constexpr int kVecs = 33;           // vectors of a lane at a time
+constexpr int kFew = 3;             // of a lane of a short share: less code to fetch
+constexpr int kGroup = 3;           // vectors between two looks at the end
+constexpr int kList = 256;          // tokens that are ranked at once
+constexpr int kKept = 64;           // vectors that are kept for it
+constexpr int kMaxCtas = 8;         // of a cluster
 constexpr int kMaxTop = YAPD_LOGPROBS_MAX_TOP;
 
 using Key = unsigned long long;  // (logit, lower id first) in ascending order; 0: none
 
 struct Logprobs {
   yapd_logprobs_args a;
+  int warps;  // of a row: 1, or kWarps times the cluster's CTAs
 };
 
 __device__ __forceinline__ Key key_of(float f, uint32_t id) {
@@ -101,20 +107,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Sums of a part of a row against its own maximum.
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Sums over a part of a row against its own maximum: z = sum e^(x - m), w = sum e^(x - m) (x - m).
 struct Part {
   float m, z, w;
 };
 // `b` joins `a`: both against the larger maximum.
 __device__ __forceinline__ Part join(const Part& a, const Part& b) {
-  Part r;
-  r.m = fmaxf(a.m, b.m);
-  if (r.m == -INFINITY) return Part{r.m, a.z + b.z, a.w + b.w};
-  const float da = fmaxf(a.m - r.m, -1e30f), db = fmaxf(b.m - r.m, -1e30f);  // a factor of 0 and not of NaN
-  const float fa = expf(da), fb = expf(db);
-  r.z = fmaf(fa, a.z, fb * b.z);
-  r.w = fa * fmaf(da, a.z, a.w) + fb * fmaf(db, b.z, b.w);
-  return r;
+  const bool left = a.m >= b.m;
+  const Part &big = left ? a : b, &small = left ? b : a;
+  if (small.m == -INFINITY) return Part{big.m, a.z + b.z, a.w + b.w};
+  const float d = fmaxf(small.m - big.m, -1e30f), f = expf(d);
+  return Part{big.m, fmaf(f, small.z, big.z), fmaf(f, fmaf(d, small.z, small.w), big.w)};
 }
 
 // A row's vectors: its first one begins at the 16-byte boundary at or below the
@@ -124,7 +133,7 @@ struct Row {
   static constexpr int kVec = 16 / (int)sizeof(T);
   const uint4* base;
   const T* x;
-  int lead, V, vectors;  // elements of the first vector before the row
+  int lead, V, vectors;  // lead: elements of the first vector before the row
 
   __device__ Row(const yapd_logprobs_args& a, int r) {
     x = (const T*)a.logits + (int64_t)r * a.stride_row;
@@ -133,10 +142,9 @@ struct Row {
     V = a.V;
     vectors = (V + lead + kVec - 1) / kVec;
   }
-  // Vector j; what is not of the row is hidden, and not read.
-  __device__ uint4 get(int j) const {
+  // A vector that ends outside the row: what is not of the row is hidden, and not read.
+  __device__ uint4 edge(int j) const {
     const int first = j * kVec - lead;
-    if (first >= 0 && first + kVec <= V) return __ldg(base + j);
     union {
       uint4 v;
       T e[kVec];
@@ -149,249 +157,360 @@ struct Row {
   }
 };
 
-struct Shared {
-  float bucket[kBuckets];
-  float z[kThreads / 32], w[kThreads / 32];
-  float threshold;
-  int listed;
-  Key list[kList];
-  // what the cluster's first CTA reads of this one
-  Part part;
-  Key top[kMaxTop];
-  Key all[kMaxCluster * kMaxTop];
-  Key best[kThreads / 32];
-};
-
-// Ranks `n` keys of `from`, all different: the k-th largest to to[k], k < most.
-__device__ __forceinline__ void rank(const Key* from, int n, Key* to, int most) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const Key mine = from[i];
-    int above = 0;
-    for (int j = 0; j < n; ++j) above += from[j] > mine;
-    if (mine && above < most) to[above] = mine;
+// Element e of a word.
+template <class T>
+__device__ __forceinline__ float word_part(uint32_t w, int e) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(w);
+  } else {
+    const float2 f = Pairs<T>::get(make_uint4(w, 0, 0, 0), 0);
+    return e ? f.y : f.x;
   }
 }
 
-template <class T, bool kOnce, bool kTop>
-__global__ void __launch_bounds__(kThreads, 4) row_kernel(const __grid_constant__ Logprobs p) {
-  __shared__ Shared sh;
-  const yapd_logprobs_args& a = p.a;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = cluster.num_blocks(), me = cluster.block_rank();
-  const int r = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Row<T> row(a, r);
-  constexpr int kVec = Row<T>::kVec, kPairs = Pairs<T>::kCount, kTile = kThreads * kVecs;
-  const int share = (row.vectors + ctas - 1) / ctas, v0 = me * share, v1 = min(v0 + share, row.vectors);
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+  return x;
+}
 
+// Vectors of a row in a warp's registers, the k-th of a lane k * 32 + lane from v0 on.
+template <class T, int kVecs>
+struct Tile {
+  static constexpr int kVec = Row<T>::kVec, kPairs = Pairs<T>::kCount;
   uint4 x[kVecs];
-  auto load = [&](int first) {
+  int v0, v1;
+
+  __device__ __forceinline__ void load(const Row<T>& row, int from, int to) {
+    v0 = from;
+    v1 = min(to, from + kVecs * 32);
+    const int lane = threadIdx.x & 31;
+    const int inner0 = row.lead ? 1 : 0, inner1 = (row.V + row.lead) / kVec;  // vectors wholly of the row
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
-      const int j = first + k * kThreads + tid;
       const uint32_t h = Pairs<T>::hidden();
       x[k] = make_uint4(h, h, h, h);
-      if (j < v1) x[k] = row.get(j);
     }
-  };
-  // The passes convert the elements anew: kept from one to the next as 32-bit
-  // numbers they would not fit the registers.
-  auto forget = [&]() {
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k) asm volatile("" : "+r"(x[k].x), "+r"(x[k].y), "+r"(x[k].z), "+r"(x[k].w));
-  };
-  // whether any lane of the warp has a k-th vector
-  auto any = [&](int first, int k) { return first + k * kThreads + warp * 32 < v1; };
-
-  // the largest logit, by thread, by four threads, of all
-  uint32_t word = Pairs<T>::hidden();
-  for (int first = v0; first < v1; first += kTile) {
-    load(first);
+    for (int g = 0; g < kVecs; g += kGroup)
+      if (v0 + g * 32 < v1)
 #pragma unroll
-    for (int k = 0; k < kVecs; ++k)
-      if (any(first, k))
-        word = Pairs<T>::larger(word, Pairs<T>::larger(Pairs<T>::larger(x[k].x, x[k].y), Pairs<T>::larger(x[k].z, x[k].w)));
-  }
-  const float mine = Pairs<T>::largest(word);
-  float top = fmaxf(mine, __shfl_xor_sync(~0u, mine, 1));
-  top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-  if ((lane & 3) == 0) sh.bucket[tid >> 2] = top;
-  if (tid == 0) {
-    sh.listed = 0;
-    sh.threshold = -INFINITY;
-  }
-  __syncthreads();
-  float m = fmaxf(sh.bucket[lane], sh.bucket[lane + 32]);
+        for (int k = g; k < g + kGroup; ++k) {
+          const int j = v0 + k * 32 + lane;
+          if (j >= inner0 && j < min(inner1, v1)) x[k] = __ldg(row.base + j);
+        }
+    // the row's first and last vector, if they are here and begin before it or end after it
+    if (v0 == 0 && v1 > 0 && inner0 && lane == 0) x[0] = row.edge(0);
+    if (inner1 < row.vectors && inner1 >= max(v0, inner0) && inner1 < v1 && lane == (inner1 - v0) % 32) {
+      const uint4 e = row.edge(inner1);
 #pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-  if (kTop) {
-    // the four threads of a bucket compare it with a quarter of the others each
-    int above = 0;
-#pragma unroll
-    for (int j = 0; j < kBuckets / 4; ++j) {
-      const int o = j * 4 + (tid & 3);
-      const float f = sh.bucket[o];
-      above += f > top || (f == top && o < tid >> 2);
+      for (int k = 0; k < kVecs; ++k)
+        if (k == (inner1 - v0) / 32) x[k] = e;
     }
-    above += __shfl_xor_sync(~0u, above, 1);
-    above += __shfl_xor_sync(~0u, above, 2);
-    if (above == a.top_n - 1) sh.threshold = top;
-    __syncthreads();
   }
 
-  // sums, and the tokens that reach the threshold
-  const float reach = kTop ? sh.threshold : 0.0f, base = m == -INFINITY ? 0.0f : m;
-  unsigned long long z2 = 0, w2 = 0;  // two sums each, for the even and the odd elements
-  const unsigned long long minus = yapd::f2_pack(-base, -base), log2e = yapd::f2_pack(yapd::kLog2e, yapd::kLog2e);
-  for (int first = v0; first < v1; first += kTile) {
-    if (!kOnce) load(first);
-    forget();
-#pragma unroll
-    for (int k = 0; k < kVecs; ++k)
-      if (any(first, k))
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          const float2 f = Pairs<T>::get(x[k], i);
-          float dx, dy, tx, ty;
-          const unsigned long long d = yapd::f2_add(yapd::f2_pack(f.x, f.y), minus);
-          yapd::f2_unpack(d, dx, dy);
-          asm("{.reg .b64 t; mul.rn.f32x2 t, %2, %3; mov.b64 {%0, %1}, t;}" : "=f"(tx), "=f"(ty) : "l"(d), "l"(log2e));
-          const unsigned long long e = yapd::f2_pack(ex2(tx), ex2(ty));
-          z2 = yapd::f2_add(z2, e);
-          // a hidden token adds 0 and not 0 times infinity
-          w2 = yapd::f2_fma(e, yapd::f2_pack(fmaxf(dx, -1e30f), fmaxf(dy, -1e30f)), w2);
-        }
-    if (kTop) {
-      // the warp looks through the vectors of each of its threads that has a candidate
-      uint32_t some = __ballot_sync(~0u, mine >= reach && mine > -INFINITY);
-      for (; some; some &= some - 1) {
-        const int from = __ffs(some) - 1;
-#pragma unroll
-        for (int y = lane; y < kVecs * kVec; y += 32) {
-          const int j = first + y / kVec * kThreads + warp * 32 + from, id = j * kVec - row.lead + y % kVec;
-          if (j < v1 && id >= 0 && id < row.V) {
-            const float g = to_f32(row.x[id]);
-            if (g >= reach && g > -INFINITY) {
-              const int at = atomicAdd(&sh.listed, 1);
-              if (at < kList) sh.list[at] = key_of(g, id);
-            }
-          }
-        }
-      }
-    }
+  __device__ __forceinline__ static uint32_t word_of(const uint4& v) {
+    return Pairs<T>::larger(Pairs<T>::larger(v.x, v.y), Pairs<T>::larger(v.z, v.w));
   }
-  float z, w, y;
-  yapd::f2_unpack(z2, z, y);
-  z += y;
-  yapd::f2_unpack(w2, w, y);
-  w += y;
+  // The lane's largest logit.
+  __device__ __forceinline__ float largest() {
+    uint32_t word = Pairs<T>::hidden();
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    z += __shfl_xor_sync(~0u, z, d);
-    w += __shfl_xor_sync(~0u, w, d);
+    for (int g = 0; g < kVecs; g += kGroup)
+      if (v0 + g * 32 < v1)
+#pragma unroll
+        for (int k = g; k < g + kGroup; ++k) word = Pairs<T>::larger(word, word_of(x[k]));
+    // 16-bit elements are converted anew: kept as 32-bit numbers they would not fit the registers.
+    if constexpr (sizeof(T) == 2)
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) asm volatile("" : "+r"(x[k].x), "+r"(x[k].y), "+r"(x[k].z), "+r"(x[k].w));
+    return Pairs<T>::largest(word);
   }
-  if (lane == 0) {
-    sh.z[warp] = z;
-    sh.w[warp] = w;
-  }
-  if (kTop && tid < kMaxTop) sh.top[tid] = 0;
-  __syncthreads();
-  if (kTop) {
-    const int n = sh.listed;
-    if (n <= kList) {
-      rank(sh.list, n, sh.top, a.top_n);
-    } else {
-      // more equal logits than the list holds: the largest below the last one, one by one
-      Key last = ~0ull;
-      for (int k = 0; k < a.top_n; ++k) {
-        Key best = 0;
-#pragma unroll 1
-        for (int j = v0 + tid; j < v1; j += kThreads) {
-          const uint4 v = row.get(j);
+  // Adds the lane's sums against `base`: two each, for the even and the odd elements.
+  __device__ __forceinline__ void add(float base, unsigned long long& z2, unsigned long long& w2) const {
+    const unsigned long long minus = yapd::f2_pack(-base, -base), log2e = yapd::f2_pack(yapd::kLog2e, yapd::kLog2e);
+#pragma unroll
+    for (int g = 0; g < kVecs; g += kGroup)
+      if (v0 + g * 32 < v1)
+#pragma unroll
+        for (int k = g; k < g + kGroup; ++k)
 #pragma unroll
           for (int i = 0; i < kPairs; ++i) {
-            const float2 f = Pairs<T>::get(v, i);
-            const Key c = key_of(f.x, j * kVec - row.lead + 2 * i), d = key_of(f.y, j * kVec - row.lead + 2 * i + 1);
-            if (f.x > -INFINITY && c < last && c > best) best = c;
-            if (f.y > -INFINITY && d < last && d > best) best = d;
+            const float2 f = Pairs<T>::get(x[k], i);
+            float dx, dy, tx, ty;
+            const unsigned long long d = yapd::f2_add(yapd::f2_pack(f.x, f.y), minus);
+            yapd::f2_unpack(d, dx, dy);
+            yapd::f2_unpack(f2_mul(d, log2e), tx, ty);
+            const unsigned long long e = yapd::f2_pack(ex2(tx), ex2(ty));
+            z2 = yapd::f2_add(z2, e);
+            // a hidden token adds 0 and not 0 times infinity
+            w2 = yapd::f2_fma(e, yapd::f2_pack(fmaxf(dx, -1e30f), fmaxf(dy, -1e30f)), w2);
           }
-        }
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-          const Key o = __shfl_xor_sync(~0u, best, d);
-          best = o > best ? o : best;
-        }
-        if (lane == 0) sh.best[warp] = best;
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < kThreads / 32; ++v) best = sh.best[v] > best ? sh.best[v] : best;
-        if (tid == 0) sh.top[k] = best;
-        last = best;
-        __syncthreads();
-      }
-    }
   }
-  if (tid == 0) {
-    Part part{m, 0.0f, 0.0f};
+  // Calls f(vector, its number) for each vector with a token that reaches `reach`.
+  template <class F>
+  __device__ __forceinline__ void reaching(float reach, F f) const {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int v = 0; v < kThreads / 32; ++v) {
-      part.z += sh.z[v];
-      part.w += sh.w[v];
-    }
-    sh.part = part;
+    for (int g = 0; g < kVecs; g += kGroup)
+      if (v0 + g * 32 < v1)
+#pragma unroll
+        for (int k = g; k < g + kGroup; ++k) {
+          const float most = Pairs<T>::largest(word_of(x[k]));
+          if (most >= reach && most > -INFINITY) f(x[k], v0 + k * 32 + lane);
+        }
   }
+};
 
-  // the cluster's first CTA puts the row together
-  const Key* best = sh.top;
-  Part all;
-  if (ctas > 1) {
-    cluster.sync();
-    if (me == 0) {
-      if (kTop) {
-        for (int i = tid; i < ctas * a.top_n; i += kThreads)
-          sh.all[i] = cluster.map_shared_rank(&sh, i / a.top_n)->top[i % a.top_n];
-        __syncthreads();
-        if (tid < kMaxTop) sh.list[tid] = 0;
-        __syncthreads();
-        rank(sh.all, ctas * a.top_n, sh.list, a.top_n);
-        best = sh.list;
-      }
-      all = sh.part;
-      for (int o = 1; o < ctas; ++o) all = join(all, cluster.map_shared_rank(&sh, o)->part);
-    }
-    cluster.sync();  // the others' memory lives until here
-    if (me != 0) return;
-  } else {
-    __syncthreads();
-    all = sh.part;
+// The warp's sums from its lanes'.
+__device__ __forceinline__ Part warp_part(float m, unsigned long long z2, unsigned long long w2) {
+  Part p{m, 0.0f, 0.0f};
+  float y;
+  yapd::f2_unpack(z2, p.z, y);
+  p.z += y;
+  yapd::f2_unpack(w2, p.w, y);
+  p.w += y;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    p.z += __shfl_xor_sync(~0u, p.z, d);
+    p.w += __shfl_xor_sync(~0u, p.w, d);
   }
+  return p;
+}
+
+// What the threads of a row put together for its alternatives: a warp's, or a CTA's.
+struct Candidates {
+  uint4 data[kKept];
+  int number[kKept];   // of the vector
+  Key list[kList];
+  Key top[kMaxTop];
+  int vectors, count;  // as many as reach the threshold, held or not
+};
+
+// The n largest of `count` keys, in their order, to `top`: all different (but
+// for 0, none), each one's place is the number of those above it.
+template <int kSize>
+__device__ __forceinline__ void place(const Key* keys, int count, int n, Key* top, int rank) {
+  for (int i = rank; i < count; i += kSize) {
+    const Key k = keys[i];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < count; ++j) above += keys[j] > k;
+    if (k && above < n) top[above] = k;
+  }
+}
+
+// The most likely tokens of vectors [v0, v1) of a row, by `kSize` threads that
+// `sync` brings together: to c.top. `tile(f)` calls f for the vectors that reach
+// `reach`, the n-th largest maximum of 32 parts.
+template <class T, int kSize, class Sync, class Tiles>
+__device__ __forceinline__ void find_top(const Row<T>& row, int v0, int v1, int n, float reach, Candidates& c, int rank,
+                                         Sync sync, Tiles tiles) {
+  constexpr int kWord = 4 / (int)sizeof(T), kVec = Row<T>::kVec;
+  if (rank < kMaxTop) c.top[rank] = 0;
+  if (rank == 0) c.vectors = c.count = 0;
+  sync();
+  tiles([&](const uint4& v, int j) {
+    const int at = atomicAdd(&c.vectors, 1);
+    if (at < kKept) {
+      c.data[at] = v;
+      c.number[at] = j;
+    }
+  });
+  sync();
+  // their tokens, a word of a vector to a thread
+  for (int i = rank; i < min(c.vectors, kKept) * 4; i += kSize) {
+    const uint32_t word = ((const uint32_t*)c.data)[i];
+    const int id = c.number[i >> 2] * kVec - row.lead + (i & 3) * kWord;
+#pragma unroll
+    for (int e = 0; e < kWord; ++e) {
+      const float g = word_part<T>(word, e);
+      if (g >= reach && g > -INFINITY) {
+        const int at = atomicAdd(&c.count, 1);
+        if (at < kList) c.list[at] = key_of(g, id + e);
+      }
+    }
+  }
+  sync();
+  if (c.vectors <= kKept && c.count <= kList) {
+    place<kSize>(c.list, c.count, n, c.top, rank);
+    sync();
+    return;
+  }
+  // more of them than are held: the largest one below the last, one by one
+  Key last = ~0ull;
+  for (int k = 0; k < n; ++k) {
+    Key best = 0;
+    for (int j = v0 + rank; j < v1; j += kSize)
+      for (int i = 0; i < kVec; ++i) {
+        const int id = j * kVec - row.lead + i;
+        const float g = id >= 0 && id < row.V ? to_f32(row.x[id]) : -INFINITY;
+        const Key x = key_of(g, id);
+        if (g > -INFINITY && x < last && x > best) best = x;
+      }
+    if (rank == 0) c.top[k] = 0;
+    sync();
+    atomicMax(&c.top[k], best);
+    sync();
+    last = c.top[k];
+  }
+}
+
+// A row's values, by the warp that holds its sums and its tokens.
+template <class T>
+__device__ __forceinline__ void write(const yapd_logprobs_args& a, const Row<T>& row, int r, const Part& all, Key top) {
+  const int lane = threadIdx.x & 31;
   // NaN or +inf make z NaN; nothing but -inf leaves no maximum
   const bool fine = all.m > -INFINITY && all.z > 0.0f && all.z < INFINITY;
   const float lz = logf(all.z);
-  if (tid == 0) {
+  if (lane == 0) {
     if (a.targets) {
       const int64_t t = a.targets[r];
       a.logprob[r] = fine && t >= 0 && t < a.V ? to_f32(row.x[t]) - all.m - lz : NAN;
     }
     if (a.entropy) a.entropy[r] = fine ? lz - all.w / all.z : NAN;
   }
-  if (kTop && tid < a.top_n) {
-    const Key k = best[tid];
-    a.top_ids[(int64_t)r * a.top_n + tid] = fine && k ? id_of(k) : -1;
-    a.top_logprobs[(int64_t)r * a.top_n + tid] = !fine ? NAN : k ? logit_of(k) - all.m - lz : -INFINITY;
+  if (lane < a.top_n) {
+    a.top_ids[(int64_t)r * a.top_n + lane] = fine && top ? id_of(top) : -1;
+    a.top_logprobs[(int64_t)r * a.top_n + lane] = !fine ? NAN : top ? logit_of(top) - all.m - lz : -INFINITY;
   }
 }
 
+// Rows of one tile: a warp to each.
+template <class T, bool kTop, int kVecs>
+__global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_constant__ Logprobs p) {
+  __shared__ Candidates candidates[kTop ? kWarps : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x * kWarps + warp; r < p.a.R; r += (int64_t)gridDim.x * kWarps) {
+    const Row<T> row(p.a, (int)r);
+    Tile<T, kVecs> tile;
+    tile.load(row, 0, row.vectors);
+    const float mine = tile.largest(), m = warp_max(mine);
+    unsigned long long z2 = 0, w2 = 0;
+    tile.add(m == -INFINITY ? 0.0f : m, z2, w2);
+    Key top = 0;
+    if (kTop) {
+      const int n = p.a.top_n;
+      const float reach = __shfl_sync(~0u, yapd::warp_bitonic_asc_f(mine), 32 - n);
+      Candidates& c = candidates[warp];
+      find_top<T, 32>(row, 0, row.vectors, n, reach, c, lane, [] { __syncwarp(); }, [&](auto f) { tile.reaching(reach, f); });
+      top = c.top[lane];
+    }
+    write(p.a, row, (int)r, warp_part(m, z2, w2), top);
+    __syncwarp();
+  }
+}
+
+struct Meeting {
+  float mine[kThreads];
+  Part part[kWarps];
+  Part all;          // what the cluster's first CTA reads of this one, with c.top
+  Part parts[kMaxCtas];
+  Candidates c;
+  Key lists[kMaxCtas * kMaxTop];
+  Key sorted[kMaxTop];
+};
+
+// A cluster to each row, a warp to each share of its vectors. kOnce: a tile holds the share.
+template <class T, bool kTop, int kVecs, bool kOnce>
+__global__ void __launch_bounds__(kThreads, kFit) row_kernel(const __grid_constant__ Logprobs p) {
+  __shared__ Meeting mt;
+  const yapd_logprobs_args& a = p.a;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = cluster.num_blocks(), me = cluster.block_rank(), n = a.top_n;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x / ctas;
+  const Row<T> row(a, r);
+  const int share = (row.vectors + p.warps - 1) / p.warps;
+  const auto first = [&](int w) { return min((me * kWarps + w) * share, row.vectors); };
+  const int v0 = first(warp), v1 = first(warp + 1);
+  Tile<T, kVecs> tile;
+  // f() for each tile of the share
+  const auto tiles = [&](auto f) {
+    if (kOnce) {
+      f();
+    } else {
+      for (int v = v0; v < v1; v += kVecs * 32) {
+        tile.load(row, v, v1);
+        f();
+      }
+    }
+  };
+  if (kOnce) tile.load(row, v0, v1);
+  float mine = -INFINITY;
+  tiles([&] { mine = fmaxf(mine, tile.largest()); });
+  if (kTop) mt.mine[tid] = mine;
+  const float m = warp_max(mine);
+  unsigned long long z2 = 0, w2 = 0;
+  tiles([&] { tile.add(m == -INFINITY ? 0.0f : m, z2, w2); });
+  Part part = warp_part(m, z2, w2);
+  if (lane == 0) mt.part[warp] = part;
+  __syncthreads();
+  if (kTop) {
+    float bucket = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) bucket = fmaxf(bucket, mt.mine[w * 32 + lane]);
+    const float reach = __shfl_sync(~0u, yapd::warp_bitonic_asc_f(bucket), 32 - n);
+    find_top<T, kThreads>(row, first(0), first(kWarps), n, reach, mt.c, tid, [] { __syncthreads(); },
+                          [&](auto f) { tiles([&] { tile.reaching(reach, f); }); });
+  }
+  if (warp == 0)
+    for (int w = 1; w < kWarps; ++w) part = join(part, mt.part[w]);
+  if (ctas == 1) {
+    if (warp == 0) write(a, row, r, part, kTop ? mt.c.top[lane] : 0);
+    return;
+  }
+  if (tid == 0) mt.all = part;
+  cluster.sync();
+  if (me == 0) {
+    if (tid < ctas) mt.parts[tid] = cluster.map_shared_rank(&mt, tid)->all;
+    if (kTop) {
+      if (tid < kMaxTop) mt.sorted[tid] = 0;
+      for (int i = tid; i < ctas * n; i += kThreads) mt.lists[i] = cluster.map_shared_rank(&mt, i / n)->c.top[i % n];
+    }
+    __syncthreads();
+    if (kTop) {
+      place<kThreads>(mt.lists, ctas * n, n, mt.sorted, tid);
+      __syncthreads();
+    }
+    if (warp == 0) {
+      for (int o = 1; o < ctas; ++o) part = join(part, mt.parts[o]);
+      write(a, row, r, part, kTop ? mt.sorted[lane] : 0);
+    }
+  }
+  cluster.sync();  // the others' memory lives until here
+}
+
+// The kernel of a configuration by whether there are alternatives.
+template <class T, int kVecs>
+auto rows_kernel_of(bool top) {
+  return top ? rows_kernel<T, true, kVecs> : rows_kernel<T, false, kVecs>;
+}
+template <class T, int kVecs, bool kOnce>
+auto row_kernel_of(bool top) {
+  return top ? row_kernel<T, true, kVecs, kOnce> : row_kernel<T, false, kVecs, kOnce>;
+}
+
 template <class T>
-int launch(const Logprobs& p, cudaStream_t st) {
+int launch(Logprobs& p, cudaStream_t st) {
   const yapd_logprobs_args& a = p.a;
   const int64_t vectors = (a.V + 2 * Row<T>::kVec - 2) / Row<T>::kVec;
-  // Few rows: a cluster to each, as long as every thread has a vector of it;
-  // a row that one CTA's registers do not hold: as many as do.
+  constexpr int kSlots = 148 * kFit * kWarps;  // warps that run at once
+  // One warp where it holds the row and there are rows for half of the warps,
+  // or the row is short; else a CTA, and a cluster for so few rows that they
+  // leave half of the GPU idle, as long as every lane has four vectors. (With
+  // 384 rows of 128256: clusters of four that hold the rows take 66 us, single
+  // CTAs that read them a second time out of L2 55 us.)
+  constexpr int kTile = kVecs * 32;
+  if (vectors <= kTile && (a.R >= kSlots / 2 || vectors <= 64)) {
+    const int ctas = (a.R + kWarps - 1) / kWarps, most = 148 * kFit;
+    const auto kernel = vectors <= kFew * 32 ? rows_kernel_of<T, kFew>(a.top_n) : rows_kernel_of<T, kVecs>(a.top_n);
+    kernel<<<ctas < most ? ctas : most, kThreads, 0, st>>>(p);
+    return launched();
+  }
   int ctas = 1;
-  while (ctas < kMaxCluster && (vectors > (int64_t)ctas * kThreads * kVecs ||
-                                ((int64_t)a.R * ctas < 2 * 148 && vectors > (int64_t)ctas * kThreads)))
-    ctas *= 2;
+  while (ctas < kMaxCtas && (int64_t)a.R * ctas * kWarps < kSlots / 2 && vectors > (int64_t)ctas * kWarps * 128) ctas *= 2;
   if ((int64_t)a.R * ctas > INT32_MAX) return YAPD_ERR_BAD_SHAPE;
+  p.warps = ctas * kWarps;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.R * ctas);
   cfg.blockDim = dim3(kThreads);
@@ -401,10 +520,11 @@ int launch(const Logprobs& p, cudaStream_t st) {
   size.val.clusterDim.x = ctas;
   size.val.clusterDim.y = size.val.clusterDim.z = 1;
   cfg.attrs = &size;
-  cfg.numAttrs = 1;
-  const bool once = (vectors + ctas - 1) / ctas <= kThreads * kVecs;
-  const auto kernel = once ? a.top_n ? row_kernel<T, true, true> : row_kernel<T, true, false>
-                           : a.top_n ? row_kernel<T, false, true> : row_kernel<T, false, false>;
+  cfg.numAttrs = ctas > 1;
+  const int64_t share = (vectors + p.warps - 1) / p.warps;
+  const auto kernel = share <= kFew * 32 ? row_kernel_of<T, kFew, true>(a.top_n)
+                      : share <= kTile   ? row_kernel_of<T, kVecs, true>(a.top_n)
+                                         : row_kernel_of<T, kVecs, false>(a.top_n);
   if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return YAPD_ERR_LAUNCH;
   return launched();
 }
@@ -426,7 +546,7 @@ extern "C" int yapd_token_logprobs(const yapd_logprobs_args* args, void* stream)
   if (!a.logits || (a.targets && !a.logprob) || (a.top_n && (!a.top_logprobs || !a.top_ids)))
     return YAPD_ERR_NULL_POINTER;
   if ((uintptr_t)a.logits % dtype_size(a.logits_dtype)) return YAPD_ERR_MISALIGNED;
-  const Logprobs p{a};
+  Logprobs p{a, 1};
   switch (a.logits_dtype) {
     case YAPD_DTYPE_F32: return launch<float>(p, (cudaStream_t)stream);
     case YAPD_DTYPE_F16: return launch<__half>(p, (cudaStream_t)stream);
