@@ -179,7 +179,9 @@ template <class T, int kVecs>
 struct Tile {
   static constexpr int kVec = Row<T>::kVec, kPairs = Pairs<T>::kCount;
   uint4 x[kVecs];
-  int v0, v1;
+  uint4 rim;  // lane 0: the row's first vector if it begins before it; lane 1: its last if it ends after it
+  int v0, v1, end;
+  bool rimmed;  // whether a lane has one
 
   __device__ __forceinline__ void load(const Row<T>& row, int from, int to) {
     v0 = from;
@@ -199,14 +201,11 @@ struct Tile {
           const int j = v0 + k * 32 + lane;
           if (j >= inner0 && j < min(inner1, v1)) x[k] = __ldg(row.base + j);
         }
-    // the row's first and last vector, if they are here and begin before it or end after it
-    if (v0 == 0 && v1 > 0 && inner0 && lane == 0) x[0] = row.edge(0);
-    if (inner1 < row.vectors && inner1 >= max(v0, inner0) && inner1 < v1 && lane == (inner1 - v0) % 32) {
-      const uint4 e = row.edge(inner1);
-#pragma unroll
-      for (int k = 0; k < kVecs; ++k)
-        if (k == (inner1 - v0) / 32) x[k] = e;
-    }
+    const bool head = v0 == 0 && v1 > 0 && inner0, tail = inner1 < row.vectors && inner1 >= max(v0, inner0) && inner1 < v1;
+    rimmed = head || tail;
+    end = inner1;
+    rim = make_uint4(Pairs<T>::hidden(), Pairs<T>::hidden(), Pairs<T>::hidden(), Pairs<T>::hidden());
+    if ((head && lane == 0) || (tail && lane == 1)) rim = row.edge(lane == 0 ? 0 : inner1);
   }
 
   __device__ __forceinline__ static uint32_t word_of(const uint4& v) {
@@ -220,6 +219,7 @@ struct Tile {
       if (v0 + g * 32 < v1)
 #pragma unroll
         for (int k = g; k < g + kGroup; ++k) word = Pairs<T>::larger(word, word_of(x[k]));
+    if (rimmed) word = Pairs<T>::larger(word, word_of(rim));
     // 16-bit elements are converted anew: kept as 32-bit numbers they would not fit the registers.
     if constexpr (sizeof(T) == 2)
 #pragma unroll
@@ -229,23 +229,26 @@ struct Tile {
   // Adds the lane's sums against `base`: two each, for the even and the odd elements.
   __device__ __forceinline__ void add(float base, unsigned long long& z2, unsigned long long& w2) const {
     const unsigned long long minus = yapd::f2_pack(-base, -base), log2e = yapd::f2_pack(yapd::kLog2e, yapd::kLog2e);
+    const auto one = [&](const uint4& v) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 f = Pairs<T>::get(v, i);
+        float dx, dy, tx, ty;
+        const unsigned long long d = yapd::f2_add(yapd::f2_pack(f.x, f.y), minus);
+        yapd::f2_unpack(d, dx, dy);
+        yapd::f2_unpack(f2_mul(d, log2e), tx, ty);
+        const unsigned long long e = yapd::f2_pack(ex2(tx), ex2(ty));
+        z2 = yapd::f2_add(z2, e);
+        // a hidden token adds 0 and not 0 times infinity
+        w2 = yapd::f2_fma(e, yapd::f2_pack(fmaxf(dx, -1e30f), fmaxf(dy, -1e30f)), w2);
+      }
+    };
 #pragma unroll
     for (int g = 0; g < kVecs; g += kGroup)
       if (v0 + g * 32 < v1)
 #pragma unroll
-        for (int k = g; k < g + kGroup; ++k)
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) {
-            const float2 f = Pairs<T>::get(x[k], i);
-            float dx, dy, tx, ty;
-            const unsigned long long d = yapd::f2_add(yapd::f2_pack(f.x, f.y), minus);
-            yapd::f2_unpack(d, dx, dy);
-            yapd::f2_unpack(f2_mul(d, log2e), tx, ty);
-            const unsigned long long e = yapd::f2_pack(ex2(tx), ex2(ty));
-            z2 = yapd::f2_add(z2, e);
-            // a hidden token adds 0 and not 0 times infinity
-            w2 = yapd::f2_fma(e, yapd::f2_pack(fmaxf(dx, -1e30f), fmaxf(dy, -1e30f)), w2);
-          }
+        for (int k = g; k < g + kGroup; ++k) one(x[k]);
+    if (rimmed) one(rim);
   }
   // Calls f(vector, its number) for each vector with a token that reaches `reach`.
   template <class F>
@@ -259,6 +262,8 @@ struct Tile {
           const float most = Pairs<T>::largest(word_of(x[k]));
           if (most >= reach && most > -INFINITY) f(x[k], v0 + k * 32 + lane);
         }
+    const float most = Pairs<T>::largest(word_of(rim));
+    if (most >= reach && most > -INFINITY) f(rim, lane == 0 ? 0 : end);
   }
 };
 
