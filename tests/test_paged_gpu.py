@@ -381,3 +381,56 @@ def test_window_reads_no_trimmed_page():
     out, lse = cache.attend(0, q.cuda(), k.cuda(), v.cuda(), window=40, sinks=10, return_lse=True)
     check(cache, q, out, lse, window=40, sinks=10)
     assert cache.status() == 0 and want.shape == out.shape
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_expired_waits_are_reported_and_contained(dtype):
+    """Waits that give up at once: the status says so, and the next call is exact again."""
+    lens = [3000, 5, 700, 0, 64]
+    cache, q, k, v = make(lens, dtype=TYPES[dtype], heads=4, kv_heads=2, layers=1)
+    want, want_l = cache.attend(0, q.cuda(), return_lse=True)
+    for _ in range(3):
+        cache.attend(0, q.cuda(), wait_limit_ns=-1)
+        assert cache.status() == N.YAPD_STATUS_WAIT_TIMEOUT
+        cache.clear_status()
+        out, lse = cache.attend(0, q.cuda(), return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_l) and cache.status() == 0
+
+
+def test_graph_capture_and_repeats():
+    """A tick captured into a graph gives the eager call's results, whatever ran between."""
+    lens = [100, 1, 900] + [33] * 60
+    cache, q, k, v = make(lens, heads=4, kv_heads=4, layers=1)
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    want = cache.attend(0, q, k, v)
+    out = torch.empty_like(want)
+    g = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        cache.attend(0, q, k, v, out=out)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    assert cache.status() == 0
+
+
+def test_example_runs():
+    """The example's beams share pages, stay within the window's pages, and are scored consistently."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_decode.py")
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    a, la, cache = m.run(requests=3, beams=2, prompt=40, tokens=30)
+    b, lb, _ = m.run(requests=3, beams=2, prompt=40, tokens=30)
+    assert torch.equal(a, b) and torch.equal(la, lb)         # the same seed, the same tokens
+    assert cache.status() == 0 and bool(torch.isfinite(la).all()) and bool((la < 0).all())
+    live = int((cache.refs > 0).sum())
+    assert live == int((cache.page_table >= 0).sum()) and bool((cache.refs[:live] == 1).all())
+    # a single candidate needs no fork
+    one, l1, _ = m.run(requests=3, beams=1, prompt=40, tokens=30)
+    assert one.shape == a.shape
