@@ -10,8 +10,8 @@
 // heads of one request, and every CTA takes the same number of consecutive
 // units, whatever the requests' lengths.  A (request, head group) that one CTA
 // holds whole is written by it; one that is cut leaves a triple per CTA in the
-// workspace, and the CTA that arrives last joins them in their order.  No CTA
-// waits for another one.
+// workspace, which a second kernel joins in their order.  No CTA waits for
+// another one.
 #include <cuda.h>  // CUtensorMap and the encode signature (the driver is reached at run time)
 
 #include <atomic>
@@ -28,7 +28,13 @@ constexpr int kWarps = 4;                     // that multiply; one more fetches
 constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kMaxRows = 64;  // query rows times key heads of a unit at most
 constexpr int64_t kWaitNs = 500000000;
-constexpr int kJoin = 4;
+
+// A (request, head group, row block) that several CTAs hold parts of.
+struct Piece {
+  int b, head0, rb;
+  int parts;   // 0: none
+  int second;  // whether the first CTA's share begins with another piece
+};
 
 struct Attend {
   yapd_attend_args a;
@@ -43,8 +49,8 @@ struct Attend {
   uint32_t negate;   // sign bits of the queries to turn
   float scale_log2;  // not negative
   int64_t wait_ns;   // limit of each wait
-  int* counters;     // (gridDim): arrivals at a cut piece that starts in the CTA
-  float* partials;   // (gridDim, 2, kMaxRows, D + 2)
+  Piece* pieces;     // (gridDim): the cut piece that begins in the CTA's share
+  float* partials;   // (gridDim, 2) of (kMaxRows, D) sums and (kMaxRows, 2) maxima and sums of weights
 };
 
 // ------------------------------------------------------------ shapes by type
@@ -733,24 +739,7 @@ struct Shared {
   float m[kWarps * M], z[kWarps * M];      // maxima and sums that meet
   long long sums[kThreads / 32];
   int found[3];
-  int arrived, given_up;
-  int left;  // pieces of the share left for others to join: 1 the first, 2 the last
-};
-
-// Of a piece cut by the CTAs' shares of `chunk` units, [start, end): the first
-// CTA that holds some of it, how many do, and where each left its triples. The
-// first one's share may begin with another piece, whose place is the other one.
-struct Cut {
-  int c0, n, off;
-  __device__ Cut(long long start, long long end, long long chunk) {
-    c0 = (int)(start / chunk);
-    n = (int)((end - 1) / chunk) - c0 + 1;
-    off = start > c0 * chunk;
-  }
-  template <int kPart>
-  __device__ const float* part(const float* partials, int k) const {
-    return partials + ((int64_t)(c0 + k) * 2 + (k == 0 ? off : 0)) * kPart;
-  }
+  int given_up;
 };
 
 template <class T, int D, int M>
@@ -792,7 +781,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     }
     yapd::mbar_init(&sh.met, kWarps);
     yapd::fence_mbar_init();
-    sh.given_up = sh.left = 0;
+    sh.given_up = 0;
+    p.pieces[blockIdx.x] = Piece{0, 0, 0, 0, 0};
   }
   __syncthreads();
   long long total = 0;
@@ -1066,68 +1056,15 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
             write_row<T>(p, b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
             if (d == 0) write_lse(p, b, head0 + hi, rb * block_rows + row, m, z);
           } else {
-            float* const to = left_at + rr * (D + 2);
-            *(float2*)(to + 4 * d) = make_float2(o.x, o.y);
-            *(float2*)(to + 4 * d + 2) = make_float2(o.z, o.w);
-            if (d == 0) *(float2*)(to + D) = make_float2(m, z);
+            *(float4*)(left_at + 4 * x) = o;
+            if (d == 0) *(float2*)(left_at + kMaxRows * D + 2 * rr) = make_float2(m, z);
           }
         }
         yapd::fence_proxy_async_smem();  // the stage is a box's target again
-        if (!whole) {
-          const Cut cut(start, end, chunk);
-          __threadfence();
-          meet();
-          if (!ok) break;
-          if (tid == 0) {
-            sh.left |= start > u0 ? 2 : 1;
-            sh.arrived = atomicAdd(p.counters + cut.c0, 1) == cut.n - 1;
-            if (sh.arrived) p.counters[cut.c0] = 0;  // for the next call; nobody else comes
-          }
-          meet();
-          if (!ok) break;
-          if (sh.arrived) {
-            __threadfence();
-            // four parts at a time, in their order: their reads go out together
-            for (int x = tid; x < p.hg * rows_here * (D / 2); x += kWarps * 32) {
-              const int rr = x / (D / 2), d = x - rr * (D / 2), hi = rr / rows_here;
-              float m = -INFINITY, z = 0.0f;
-              float2 o = make_float2(0.0f, 0.0f);
-              for (int k0 = 0; k0 < cut.n; k0 += kJoin) {
-                float2 mz[kJoin], v[kJoin];
-#pragma unroll
-                for (int k = 0; k < kJoin; ++k) {
-                  const float* const y = cut.part<kPart>(p.partials, min(k0 + k, cut.n - 1)) + rr * (D + 2);
-                  mz[k] = __ldcg((const float2*)(y + D));
-                  v[k] = __ldcg((const float2*)(y + 2 * d));
-                }
-                float top = m;
-#pragma unroll
-                for (int k = 0; k < kJoin; ++k) top = fmaxf(top, mz[k].x);
-                const float base = top == -INFINITY ? 0.0f : top, f0 = ex2(m - base);
-                z *= f0;
-                o.x *= f0;
-                o.y *= f0;
-#pragma unroll
-                for (int k = 0; k < kJoin; ++k)
-                  if (k0 + k < cut.n) {
-                    const float f = ex2(mz[k].x - base);
-                    z = fmaf(f, mz[k].y, z);
-                    o.x = fmaf(f, v[k].x, o.x);
-                    o.y = fmaf(f, v[k].y, o.y);
-                  }
-                m = top;
-              }
-              const float rz = z == 0.0f ? 0.0f : 1.0f / z;
-              const int full = rb * block_rows + rr - hi * rows_here, i = (int)div_floor(full, p.groups);
-              const int h = (head0 + hi) * p.group + full - i * p.group;
-              T* const out = (T*)p.a.out + b * p.a.out_stride_req + i * p.a.out_stride_pos + h * p.a.out_stride_head + 2 * d;
-              if constexpr (sizeof(T) == 4)
-                *(float2*)out = make_float2(o.x * rz, o.y * rz);
-              else
-                *(uint32_t*)out = pack2<T>(o.x * rz, o.y * rz);
-              if (d == 0) write_lse(p, b, head0 + hi, full, m, z);
-            }
-          }
+        if (!whole && start >= u0 && tid == 0) {
+          // the piece begins here: where the parts are, for the kernel that joins them
+          const long long c0 = start / chunk;
+          p.pieces[blockIdx.x] = Piece{b, head0, rb, (int)((end - 1) / chunk - c0) + 1, start > u0};
         }
         fresh = true;
       }
@@ -1144,30 +1081,72 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     }
   }
 
-  // A CTA that gave up still takes part in the counts of the pieces that it
-  // shares, with sums that are no numbers, so that the counters end at zero.
+  // A CTA that gave up leaves no numbers to the pieces that it shares.
   __syncthreads();
-  if (sh.given_up && tid == 0) {
-    Cursor x;
-    x.b = sh.found[0];
-    x.hr = sh.found[1];
-    x.tile = 0;
-    enter(p, x, shift);
-    long long start = u0 - sh.found[2];
-    while (start < u1) {
-      const long long end = start + x.span.tiles;
-      const int which = start > u0 ? 2 : 1;
-      if ((start < u0 || end > u1) && !(sh.left & which)) {
-        const Cut cut(start, end, chunk);
-        float* const to = p.partials + ((int64_t)blockIdx.x * 2 + which - 1) * kPart;
-        for (int r = 0; r < kMaxRows; ++r) *(float2*)(to + r * (D + 2) + D) = make_float2(0.0f, NAN);
-        __threadfence();
-        if (atomicAdd(p.counters + cut.c0, 1) == cut.n - 1) p.counters[cut.c0] = 0;
+  if (sh.given_up)
+    for (int r = tid; r < 2 * kMaxRows; r += kThreads)
+      *(float2*)(p.partials + ((int64_t)blockIdx.x * 2 + r / kMaxRows) * kPart + kMaxRows * D + r % kMaxRows * 2) =
+          make_float2(0.0f, NAN);
+}
+
+// Joins the parts of the piece that begins in a CTA's share, in their order:
+// four dims of a row to a thread, and where that leaves threads over, the parts
+// are shared out over groups of them. Time is the latency of the reads, so a
+// thread has eight parts' under way.
+constexpr int kJoinThreads = 256;
+template <class T, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Attend p, int block_rows) {
+  constexpr int64_t kPart = kMaxRows * (D + 2);
+  __shared__ float2 mzs[kJoinThreads];
+  __shared__ float4 os[kJoinThreads];
+  const int tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Piece piece = p.pieces[blockIdx.x];
+  if (piece.parts == 0) return;
+  const int rows_here = min(block_rows, p.rows - piece.rb * block_rows), items = p.hg * rows_here * (D / 4);
+  const int groups = max(1, min(min(kJoinThreads / items, 8), piece.parts / 4));
+  const int group = groups > 1 ? tid / items : 0;
+  // the first CTA's part is its second one unless its share begins with the piece
+  const auto part_at = [&](int k) { return p.partials + ((int64_t)(blockIdx.x + k) * 2 + (k == 0 ? piece.second : 0)) * kPart; };
+  const auto add = [](float& m, float& z, float4& o, float2 mz, float4 v) {
+    const float top = fmaxf(m, mz.x), base = top == -INFINITY ? 0.0f : top, f0 = ex2(m - base), f = ex2(mz.x - base);
+    z = fmaf(f, mz.y, z * f0);
+    o.x = fmaf(f, v.x, o.x * f0);
+    o.y = fmaf(f, v.y, o.y * f0);
+    o.z = fmaf(f, v.z, o.z * f0);
+    o.w = fmaf(f, v.w, o.w * f0);
+    m = top;
+  };
+  for (int x = groups > 1 ? tid - group * items : tid; x < items; x += kJoinThreads) {
+    float m = -INFINITY, z = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = group; k0 < piece.parts && group < groups; k0 += 8 * groups) {
+      float2 mz[8];
+      float4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mz[k] = make_float2(-INFINITY, 0.0f);
+        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (k0 + k * groups < piece.parts) {
+          const float* const y = part_at(k0 + k * groups);
+          mz[k] = __ldcg((const float2*)(y + kMaxRows * D + x / (D / 4) * 2));
+          v[k] = __ldcg((const float4*)(y + 4 * x));
+        }
       }
-      start = end;
-      x.tile = x.span.tiles - 1;
-      advance(p, x, shift);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) add(m, z, o, mz[k], v[k]);
     }
+    if (groups > 1) {
+      mzs[tid] = make_float2(m, z);
+      os[tid] = o;
+      __syncthreads();  // every thread comes here once: the items are fewer than the threads
+      if (group) break;
+      for (int g = 1; g < groups; ++g) add(m, z, o, mzs[g * items + x], os[g * items + x]);
+    }
+    const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here;
+    const int full = piece.rb * block_rows + rr - hi * rows_here;
+    write_row<T>(p, piece.b, piece.head0 + hi, full, 4 * d, o, z == 0.0f ? 0.0f : 1.0f / z);
+    if (d == 0) write_lse(p, piece.b, piece.head0 + hi, full, m, z);
   }
 }
 
@@ -1254,16 +1233,21 @@ int launch(Attend& p, cudaStream_t st) {
   cfg.dynamicSmemBytes = Shape<T, D, M>::kSmem;
   cfg.stream = st;
   cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
   if (p.a.k) {
     const int rows = p.a.B * p.a.new_tokens;
     store_kernel<T><<<(rows + 3) / 4, 128, 0, st>>>(p);
     // the attention's CTAs start beside the stores and wait for them where they read the pages
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
   }
   if (cudaLaunchKernelEx(&cfg, attend_kernel<T, D, M>, p, map) != cudaSuccess) return YAPD_ERR_LAUNCH;
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p, M * p.wr) != cudaSuccess) return YAPD_ERR_LAUNCH;
   return launched();
 }
 
@@ -1292,7 +1276,7 @@ bool rows_aligned(const void* base, int64_t r, int64_t p, int64_t h, int dtype) 
 }  // namespace
 
 size_t attend_scratch_bytes(const yapd_cache& c) {
-  return round_up(kMaxCtas * 4, 256) + (size_t)kMaxCtas * 2 * kMaxRows * (c.head_dim + 2) * 4;
+  return round_up(kMaxCtas * sizeof(Piece), 256) + (size_t)kMaxCtas * 2 * kMaxRows * (c.head_dim + 2) * 4;
 }
 
 }  // namespace serve
@@ -1328,8 +1312,8 @@ extern "C" int yapd_attend(const yapd_attend_args* args, void* stream) {
   p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
   p.wait_ns = a.wait_limit_ns ? a.wait_limit_ns : kWaitNs;
   char* const scratch = (char*)a.cache.workspace + kHeaderBytes + pages_scratch_bytes(a.cache);
-  p.counters = (int*)scratch;
-  p.partials = (float*)(scratch + round_up(kMaxCtas * 4, 256));
+  p.pieces = (Piece*)scratch;
+  p.partials = (float*)(scratch + round_up(kMaxCtas * sizeof(Piece), 256));
   switch (dt) {
     case YAPD_DTYPE_F32: return launch_dim<float>(p, (cudaStream_t)stream);
     case YAPD_DTYPE_F16: return launch_dim<__half>(p, (cudaStream_t)stream);
