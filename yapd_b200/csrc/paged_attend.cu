@@ -77,8 +77,10 @@ struct Shape {
   static constexpr int kWords = kRows / 32;          // of a mask of a tile's keys
   static constexpr int kQuery = sizeof(T) == 4 ? M * (D + 4) : 0;  // floats of a warp's queries in shared memory
   static constexpr int kSmem = kStages * kStage + kWarps * kQuery * 4;
-  // CTAs of an SM: as many as its 228 KB hold, and no more than leave a thread the registers of its sums
-  static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 1024), kMost = M == 16 ? 3 : 4;
+  // CTAs of an SM: as many as its 228 KB hold, and no more than leave a thread
+  // the registers of its sums (16 rows, 128 rows of blocks: 109 us with three
+  // CTAs, 127 with two, 133 with four; in 32 bits 247 us with two, 296 with three)
+  static constexpr int kRoom = 228 * 1024 / (kSmem + 1024 + 1024), kMost = sizeof(T) == 4 ? (M == 16 ? 2 : 3) : M == 16 ? 3 : 4;
   static constexpr int kFit = kRoom < kMost ? kRoom : kMost;
   static_assert(kWarps * M * D * 4 <= kStage, "the warps' triples meet in a stage");
 
@@ -723,6 +725,22 @@ __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int 
       z == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(z);
 }
 
+// The kernel. Its bound is the rate of the pages' reads: a token's key and value
+// row, 4 D bytes at 16 bits, meet 4 D rows operations, so up to about 100 query
+// rows of a key head the products are the smaller part; they run on the
+// mma.sync pipe, whose tiles of 16 rows fit these counts (a tcgen05 tile has 64
+// or 128), at a tenth of its rate. What it took to get there, 256 requests of
+// 16 heads of 64 and 20 to 1250 tokens (692 MB; 106 us at the copy rate):
+//   every warp copying its share of a stage, 255 registers       217 us
+//   products by the number of rows, four CTAs per SM             169 us
+//   one fetching warp, a 512-byte bulk copy to a token           161 us (17 ns a copy and SM)
+//   one fetching warp, 16 bytes a lane                           184 us
+//   one fetching warp, boxes of 16 tokens                        125 us
+// and 4 requests of 95k tokens with 8 key heads of 128 (1.63 GB) 250 us, 99.9 %
+// of the copy rate. A launch with three tiles to a CTA takes 11 us: 3.3 us to the
+// first box, 1 us for a tile, 2 us for what the warps and the joining kernel add
+// up, the rest for the three launches.
+
 // What the fetching warp says of a tile.
 struct Tile {
   int b, head0, rb, len, k0;  // request, first key head, row block, tokens, first token
@@ -1218,11 +1236,13 @@ int launch(Attend& p, cudaStream_t st) {
   p.wr = M < 16 || p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
   p.row_blocks = (p.rows + M * p.wr - 1) / (M * p.wr);
   // Key heads of a unit: the rows of several heads of a token lie side by side
-  // in its page.  Few requests are shared out by heads first, so that fewer
-  // CTAs hold parts of the same sums.
+  // in its page, and a piece has more tiles (256 requests of 16 heads: 169 us
+  // with four, 182 with two, 218 with one).  Few requests are shared out by
+  // heads first, so that fewer CTAs hold parts of the same sums (64 requests:
+  // 44 us with four heads; 48 requests of 4 heads: 49 us with one, 54 with two).
   const int kvh = p.a.cache.kv_heads;
   p.hg = Shape<T, D, M>::kMaxHeads >= p.wr ? Shape<T, D, M>::kMaxHeads / p.wr : 1;
-  while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < grid / 2)) p.hg /= 2;
+  while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < grid / 4)) p.hg /= 2;
   p.head_groups = kvh / p.hg;
   CUtensorMap map{};
   p.boxes = p.a.cache.page_size % 16 == 0;
