@@ -843,12 +843,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     const int at_once = chunks >= 32 ? 1 : 32 / chunks;     // tokens of one instruction
     const int my_token = chunks >= 32 ? 0 : lane / chunks, my_chunk = lane - my_token * chunks;
     const bool copying = my_token < at_once;
+    static_assert(kChunks * S::kMaxHeads <= 64, "two chunks of a token to a lane");
     const int64_t to_v = (int64_t)c.page_size * c.kv_heads * D;
-    // bytes from the stage's start to chunk x of token y's keys
-    auto chunk_at = [&](int y, int x) {
-      const int h = x / kChunks, ch = x % kChunks, tok = y & 15;
-      return (y >> 4) * group_bytes + ((ch / kIn * p.hg + h) * 16 + tok) * S::kInner + (ch % kIn << 4 ^ S::turn(tok));
-    };
+    // where the lane's one or two chunks of a token lie in a group
+    const auto slab_of = [&](int x) { return (x % kChunks / kIn * p.hg + x / kChunks) * S::kSlab; };
+    const int chunk2 = my_chunk + 32, slab1 = slab_of(my_chunk), slab2 = slab_of(chunk2);
+    const int in1 = my_chunk % kChunks % kIn << 4, in2 = chunk2 % kChunks % kIn << 4;
+    const bool two = chunk2 < chunks;
     int entry[kPer];
     Cursor at;
     auto ask = [&]() {
@@ -937,16 +938,21 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         for (int e = 0; e < kPer; ++e) {
           const int j = k0 + lane + 32 * e, r = j - (int)div_floor(j, p.page) * c.page_size;
           const int64_t place = entry[e] == kNone ? -1 : entry[e] * c.stride_page + (int64_t)r * c.kv_heads * D;
-          for (int y0 = 0; y0 < 32 && y0 + 32 * e < keys; y0 += at_once) {
-            const int y = 32 * e + y0 + my_token;
-            const int64_t from = __shfl_sync(~0u, place, y0 + my_token);
-            const T* const k = base + from;
-            if (copying && from >= 0)
-              for (int x = my_chunk; x < chunks; x += 32) {
-                const uint32_t d = to + chunk_at(y, x);
-                copy16(d, k + x * kVec);
-                copy16(d + S::kHalf, k + to_v + x * kVec);
-              }
+          const int turns = min(32, keys - 32 * e) / at_once;
+#pragma unroll 4
+          for (int i = 0; i < turns; ++i) {
+            const int from_lane = i * at_once + my_token, y = 32 * e + from_lane, tok = y & 15;
+            const int64_t from = __shfl_sync(~0u, place, from_lane);
+            if (!copying || from < 0) continue;
+            const T* const k = base + from + my_chunk * kVec;
+            const uint32_t row = to + (y >> 4) * group_bytes + tok * S::kInner, d = row + slab1 + (in1 ^ S::turn(tok));
+            copy16(d, k);
+            copy16(d + S::kHalf, k + to_v);
+            if (two) {
+              const uint32_t d2 = row + slab2 + (in2 ^ S::turn(tok));
+              copy16(d2, k + 32 * kVec);
+              copy16(d2 + S::kHalf, k + 32 * kVec + to_v);
+            }
           }
         }
       }
@@ -1235,6 +1241,7 @@ int launch(Attend& p, cudaStream_t st) {
   if (rc != YAPD_OK) return rc;
   p.wr = M < 16 || p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
   p.row_blocks = (p.rows + M * p.wr - 1) / (M * p.wr);
+  p.boxes = p.a.cache.page_size % 16 == 0;
   // Key heads of a unit: the rows of several heads of a token lie side by side
   // in its page, and a piece has more tiles (256 requests of 16 heads: 169 us
   // with four, 182 with two, 218 with one).  Few requests are shared out by
@@ -1242,10 +1249,10 @@ int launch(Attend& p, cudaStream_t st) {
   // 44 us with four heads; 48 requests of 4 heads: 49 us with one, 54 with two).
   const int kvh = p.a.cache.kv_heads;
   p.hg = Shape<T, D, M>::kMaxHeads >= p.wr ? Shape<T, D, M>::kMaxHeads / p.wr : 1;
-  while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < grid / 4)) p.hg /= 2;
+  const int64_t pieces = p.boxes ? grid / 4 : 0;
+  while (p.hg > 1 && (kvh % p.hg || (int64_t)p.a.B * (kvh / p.hg) * p.row_blocks < pieces)) p.hg /= 2;
   p.head_groups = kvh / p.hg;
   CUtensorMap map{};
-  p.boxes = p.a.cache.page_size % 16 == 0;
   if (p.boxes && !encode<T, D, M>(p, map)) return YAPD_ERR_LAUNCH;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
