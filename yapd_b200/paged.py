@@ -82,8 +82,9 @@ class PagedCache:
             raise ValueError("page_size, kv_heads or max_pages * page_size is out of range")
         self._workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
         c.workspace, c.workspace_bytes = self._workspace.data_ptr(), need
-        self._attend, self._pages = N.AttendArgs(), N.PagesArgs()
-        self._attend.cache = self._pages.cache = c
+        self._pages = N.PagesArgs()
+        self._cache = self._pages.cache = c
+        self._scale, self._plans = self._dim ** -0.5, {}
 
     @classmethod
     def empty(cls, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int,
@@ -110,7 +111,8 @@ class PagedCache:
         ``kv_heads``; row ``b`` is slot ``slots[b]`` (int32), or slot ``b``.
         ``k`` and ``v`` (``q``'s shape with ``kv_heads``) are stored in the
         tokens' pages by the same call; without them the pages are only read.
-        The tokens are part of ``kv_len`` already (``reserve``).
+        The tokens are part of ``kv_len`` already (``reserve``).  ``out``, if given,
+        overlaps none of the inputs.
 
         Query ``i``, at position ``p = kv_len - T + i``, sees the tokens of its
         request, up to ``p`` if ``causal``, and with ``window > 0`` only those
@@ -121,22 +123,18 @@ class PagedCache:
         logarithms of the softmax's sums.  ``wait_limit_ns`` bounds each wait for
         a copy, as in ``select_step``.
         """
-        a, dtype, index = self._attend, self._dtype, self._index
-        shape = q.shape
-        if len(shape) == 3:
-            q = q.unsqueeze(1)
-            k = k if k is None or k.dim() != 3 else k.unsqueeze(1)
-            v = v if v is None or v.dim() != 3 else v.unsqueeze(1)
-        if q.dim() != 4:
-            raise ValueError(f"q must be (B, [T,] heads, {self._dim}), got {tuple(shape)}")
-        B, T, H, D = q.shape
-        if D != self._dim or H % self._heads or H == 0:
-            raise ValueError(f"q must be (B, [T,] heads, {self._dim}) with heads a multiple of {self._heads}, "
-                             f"got {tuple(shape)}")
-        if not 1 <= T <= N.YAPD_MAX_NEW_TOKENS:
-            raise ValueError(f"1 to {N.YAPD_MAX_NEW_TOKENS} new tokens, got {T}")
-        if q.dtype != dtype or q.get_device() != index:
-            raise TypeError(f"q must be {dtype} on {self.device}")
+        key = (q.shape, q.stride(), q.dtype)
+        if k is not None and v is not None:
+            key += (k.shape, k.stride(), k.dtype, v.shape, v.stride(), v.dtype)
+        elif k is not v:
+            raise ValueError("k and v come together")
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plan(key)
+        a, B, copies, shape, o, out_like, lse_like = plan
+        if q.get_device() != self._index or (k is not None and (k.get_device() != self._index or
+                                                                v.get_device() != self._index)):
+            raise TypeError(f"q, k and v must be on {self.device}")
         if not 0 <= layer < self._layers:
             raise ValueError(f"layer {layer} of {self._layers}")
         if sinks < 0:
@@ -148,35 +146,72 @@ class PagedCache:
             raise ValueError(f"{B} requests, but {self.slots} slots")
         else:
             a.slots = None
-        q, (a.q_stride_req, a.q_stride_pos, a.q_stride_head, _) = self._rows(q)
-        a.layer, a.B, a.new_tokens, a.heads, a.q = layer, B, T, H, q.data_ptr()
-        if k is None and v is None:
-            a.k = a.v = None
-        else:
-            if k is None or v is None:
-                raise ValueError("k and v come together")
-            want = (B, T, self._heads, D)
-            if k.shape != want or v.shape != want:
-                raise ValueError(f"k and v must be {want}, got {tuple(k.shape)} and {tuple(v.shape)}")
-            if k.dtype != dtype or v.dtype != dtype or k.get_device() != index or v.get_device() != index:
-                raise TypeError(f"k and v must be {dtype} on {self.device}")
-            k, (a.k_stride_req, a.k_stride_pos, a.k_stride_head, _) = self._rows(k)
-            v, (a.v_stride_req, a.v_stride_pos, a.v_stride_head, _) = self._rows(v)
+        at = q.data_ptr()
+        if copies or at % 16 or (k is not None and (k.data_ptr() % 16 or v.data_ptr() % 16)):
+            # rows that the kernels cannot read: contiguous copies
+            q = q.clone(memory_format=torch.contiguous_format)
+            if k is not None:
+                k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+            return self.attend(layer, q, k, v, slots=slots, causal=causal, window=window, sinks=sinks, scale=scale,
+                               out=out, return_lse=return_lse, wait_limit_ns=wait_limit_ns)
+        a.q = at
+        if k is not None:
             a.k, a.v = k.data_ptr(), v.data_ptr()
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=self.device) if len(shape) == 3 or not q.is_contiguous() \
-                else torch.empty_like(q)
-        elif out.shape != shape or out.dtype != dtype or out.get_device() != index or self._rows(out)[0] is not out:
-            raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor on {self.device} whose rows are aligned")
+            out = torch.empty_like(out_like)
+        else:
+            o = out.stride()
+            if out.shape != shape or out.dtype != self._dtype or out.get_device() != self._index or \
+                    out.data_ptr() % 16 or self._unreadable(o):
+                raise ValueError(f"out must be a {tuple(shape)} {self._dtype} tensor on {self.device} whose rows are aligned")
         a.out = out.data_ptr()
-        st = out.stride()
-        a.out_stride_req, a.out_stride_pos, a.out_stride_head = st[:3] if len(st) == 4 else (st[0], 0, st[1])
-        lse = torch.empty(shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
+        a.out_stride_req, a.out_stride_pos, a.out_stride_head = (o[0], 0, o[1]) if len(o) == 3 else o[:3]
+        lse = torch.empty_like(lse_like) if return_lse else None
         a.lse = lse.data_ptr() if return_lse else None
-        a.scale = D ** -0.5 if scale is None else scale
+        a.layer, a.scale = layer, self._scale if scale is None else scale
         a.causal, a.window, a.sinks, a.wait_limit_ns = 1 if causal else 0, window, sinks, wait_limit_ns
         self._call(self._lib.yapd_attend, a)
         return (out, lse) if return_lse else out
+
+    def _unreadable(self, strides) -> bool:
+        """Whether the kernels cannot read rows with these strides."""
+        return strides[-1] != 1 or any(s % self._vec for s in strides[:-1])
+
+    def _plan(self, key):
+        """The checks of an attention call's shapes, strides and types, and its
+        arguments as far as they follow from them: kept, for the layers of a
+        tick and the ticks of a batch are alike."""
+        shape, stride, dtype = key[:3]
+        if len(shape) not in (3, 4) or shape[-1] != self._dim or shape[-2] % self._heads or shape[-2] == 0:
+            raise ValueError(f"q must be (B, [T,] heads, {self._dim}) with heads a multiple of {self._heads}, "
+                             f"got {tuple(shape)}")
+        B, T, H, D = shape if len(shape) == 4 else (shape[0], 1, *shape[1:])
+        if not 1 <= T <= N.YAPD_MAX_NEW_TOKENS:
+            raise ValueError(f"1 to {N.YAPD_MAX_NEW_TOKENS} new tokens, got {T}")
+        if dtype != self._dtype:
+            raise TypeError(f"q must be {self._dtype}, got {dtype}")
+        a = N.AttendArgs()
+        a.cache = self._cache
+        a.B, a.new_tokens, a.heads = B, T, H
+        three = lambda st: (st[0], 0, st[1]) if len(st) == 3 else st[:3]  # noqa: E731
+        a.q_stride_req, a.q_stride_pos, a.q_stride_head = three(stride)
+        copies = self._unreadable(stride)
+        if len(key) > 3:
+            want = (*shape[:-2], self._heads, D)
+            if tuple(key[3]) != want or tuple(key[6]) != want:
+                raise ValueError(f"k and v must be {want}, got {tuple(key[3])} and {tuple(key[6])}")
+            if key[5] != self._dtype or key[8] != self._dtype:
+                raise TypeError(f"k and v must be {self._dtype}")
+            a.k_stride_req, a.k_stride_pos, a.k_stride_head = three(key[4])
+            a.v_stride_req, a.v_stride_pos, a.v_stride_head = three(key[7])
+            copies = copies or self._unreadable(key[4]) or self._unreadable(key[7])
+        if len(self._plans) >= 64:
+            self._plans.clear()
+        # one element seen in the outputs' shapes: torch.empty_like costs half of torch.empty
+        like = lambda dtype, shape: torch.empty(1, dtype=dtype, device=self.device).expand(shape)  # noqa: E731
+        out_like, lse_like = like(self._dtype, shape), like(torch.float32, shape[:-1])
+        self._plans[key] = plan = (a, B, copies, shape, torch.empty_like(out_like).stride(), out_like, lse_like)
+        return plan
 
     # ----------------------------------------------------------------- pages
 
@@ -257,16 +292,6 @@ class PagedCache:
         N.check(self._lib.yapd_clear_status(C.c_void_p(self._workspace.data_ptr()), self._stream()))
 
     # --------------------------------------------------------------- private
-
-    def _rows(self, t: torch.Tensor):
-        """``t`` and its strides if the kernels can read its rows of the last
-        dimension, else those of a contiguous copy."""
-        st = t.stride()
-        vec = self._vec
-        if st[-1] != 1 or t.data_ptr() % 16 or st[0] % vec or st[1] % vec or st[-2] % vec:
-            t = t.clone(memory_format=torch.contiguous_format)
-            st = t.stride()
-        return t, st
 
     def _stream(self) -> int:
         return torch._C._cuda_getCurrentRawStream(self._index)
