@@ -1149,8 +1149,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       float4 v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        mz[k] = make_float2(-INFINITY, 0.0f);
-        v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (k0 + k * groups < piece.parts) {
           const float* const y = part_at(k0 + k * groups);
           mz[k] = __ldcg((const float2*)(y + kMaxRows * D + x / (D / 4) * 2));
@@ -1158,7 +1156,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         }
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) add(m, z, o, mz[k], v[k]);
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k * groups < piece.parts) add(m, z, o, mz[k], v[k]);
     }
     if (groups > 1) {
       mzs[tid] = make_float2(m, z);

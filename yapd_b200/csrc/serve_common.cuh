@@ -46,7 +46,7 @@ __device__ __forceinline__ uint32_t div_floor(uint32_t t, const Div& v) {
 // ---------------------------------------------------------------- the cache
 
 // Workspace: the status word, then integer scratch of the page operations,
-// then the attention's (its counters first, which stay zero between calls).
+// then the attention's.
 constexpr size_t kHeaderBytes = 256;
 // Attention: CTAs of one launch at most, and the floats that one of them may
 // leave for others to join.
