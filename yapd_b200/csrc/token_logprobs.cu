@@ -26,6 +26,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kFit = 3;             // CTAs of an SM: 168 registers a thread
 constexpr int kVecs = 33;           // vectors of a lane at a time
+constexpr int kSome = 18;           // of a lane of a longer row's share, four CTAs to an SM
+constexpr int kSomeFit = 4;
 constexpr int kFew = 3;             // of a lane of a short share: less code to fetch
 constexpr int kGroup = 3;           // vectors between two looks at the end
 constexpr int kList = 256;          // tokens that are ranked at once
@@ -381,7 +383,11 @@ __device__ __forceinline__ void write(const yapd_logprobs_args& a, const Row<T>&
   }
 }
 
-// Rows of one tile: a warp to each.
+// Rows of one tile: a warp to each, nothing to wait for. 8192 rows of 8194 16-bit
+// logits (134 MB; 21 us at the copy rate) take 35 us, with eight alternatives 51
+// us: 2400 and 3200 instructions a row at half of the issue slots, since a row in
+// registers leaves room for twelve warps to an SM. Four warps to such a row: 36
+// and 53 us; a block of 256 threads: 49 and 77 us.
 template <class T, bool kTop, int kVecs>
 __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_constant__ Logprobs p) {
   __shared__ Candidates candidates[kTop ? kWarps : 1];
@@ -416,9 +422,13 @@ struct Meeting {
   Key sorted[kMaxTop];
 };
 
-// A cluster to each row, a warp to each share of its vectors. kOnce: a tile holds the share.
+// A CTA or a cluster to each row, a warp to each share of its vectors. kOnce: a
+// tile holds the share. 4096 rows of 8192 32-bit logits (134 MB) take 29 us, 71 % of
+// the copy rate; 384 rows of 128256 16-bit ones,
+// read twice, take 52 us (15 us at the copy rate), of which the alternatives are
+// 14; one row of 6563 takes 6 us, two meetings of the cluster's CTAs and launch.
 template <class T, bool kTop, int kVecs, bool kOnce>
-__global__ void __launch_bounds__(kThreads, kFit) row_kernel(const __grid_constant__ Logprobs p) {
+__global__ void __launch_bounds__(kThreads, kSomeFit) row_kernel(const __grid_constant__ Logprobs p) {
   __shared__ Meeting mt;
   const yapd_logprobs_args& a = p.a;
   const cg::cluster_group cluster = cg::this_cluster();
@@ -504,7 +514,8 @@ int launch(Logprobs& p, cudaStream_t st) {
   // or the row is short; else a CTA, and a cluster for so few rows that they
   // leave half of the GPU idle, as long as every lane has four vectors. (With
   // 384 rows of 128256: clusters of four that hold the rows take 66 us, single
-  // CTAs that read them a second time out of L2 55 us.)
+  // CTAs that read them a second time out of L2 52 us; 4096 rows of 8192 in 32
+  // bits: 29 us with 18 vectors to a lane, 37 with 33, 33 with 9.)
   constexpr int kTile = kVecs * 32;
   if (vectors <= kTile && (a.R >= kSlots / 2 || vectors <= 64)) {
     const int ctas = (a.R + kWarps - 1) / kWarps, most = 148 * kFit;
@@ -513,7 +524,7 @@ int launch(Logprobs& p, cudaStream_t st) {
     return launched();
   }
   int ctas = 1;
-  while (ctas < kMaxCtas && (int64_t)a.R * ctas * kWarps < kSlots / 2 && vectors > (int64_t)ctas * kWarps * 128) ctas *= 2;
+  while (ctas < kMaxCtas && (int64_t)a.R * ctas < 148 * kSomeFit / 2 && vectors > (int64_t)ctas * kWarps * 128) ctas *= 2;
   if ((int64_t)a.R * ctas > INT32_MAX) return YAPD_ERR_BAD_SHAPE;
   p.warps = ctas * kWarps;
   cudaLaunchConfig_t cfg{};
@@ -528,8 +539,8 @@ int launch(Logprobs& p, cudaStream_t st) {
   cfg.numAttrs = ctas > 1;
   const int64_t share = (vectors + p.warps - 1) / p.warps;
   const auto kernel = share <= kFew * 32 ? row_kernel_of<T, kFew, true>(a.top_n)
-                      : share <= kTile   ? row_kernel_of<T, kVecs, true>(a.top_n)
-                                         : row_kernel_of<T, kVecs, false>(a.top_n);
+                      : share <= kSome * 32 ? row_kernel_of<T, kSome, true>(a.top_n)
+                                            : row_kernel_of<T, kSome, false>(a.top_n);
   if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return YAPD_ERR_LAUNCH;
   return launched();
 }
