@@ -775,6 +775,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
   const int pairs = p.head_groups * p.row_blocks;
   const int group_bytes = p.hg * 16 * S::kBytes;
 
+  // every CTA of the grid runs: those of the joining kernel may take the place of the ones that end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // all units, and where this CTA's share begins
   const int per = (p.a.B + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.a.B), b1 = min(b0 + per, p.a.B);
