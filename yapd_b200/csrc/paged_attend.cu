@@ -669,6 +669,22 @@ __global__ void __launch_bounds__(128) store_kernel(const __grid_constant__ Atte
   const int lane = threadIdx.x & 31, x = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (x >= p.a.B * p.a.new_tokens) return;
   const int b = x / p.a.new_tokens, i = x - b * p.a.new_tokens;
+  // the first rows are on their way while their place is looked up
+  constexpr int kVec = 16 / sizeof(T), kFirst = 4;
+  const int per = c.head_dim / kVec, all = c.kv_heads * per;
+  const T* const k = (const T*)p.a.k + b * p.a.k_stride_req + i * p.a.k_stride_pos;
+  const T* const v = (const T*)p.a.v + b * p.a.v_stride_req + i * p.a.v_stride_pos;
+  const auto row = [&](const T* rows, int64_t stride_head, int y) {
+    const int h = y / per;
+    return *(const uint4*)(rows + h * stride_head + (y - h * per) * kVec);
+  };
+  uint4 kx[kFirst], vx[kFirst];
+#pragma unroll
+  for (int u = 0; u < kFirst; ++u)
+    if (lane + 32 * u < all) {
+      kx[u] = row(k, p.a.k_stride_head, lane + 32 * u);
+      vx[u] = row(v, p.a.v_stride_head, lane + 32 * u);
+    }
   int slot;
   const int t = slot_len(p, b, slot) - p.a.new_tokens + i;
   uint32_t wrong = 0;
@@ -689,19 +705,20 @@ __global__ void __launch_bounds__(128) store_kernel(const __grid_constant__ Atte
     if (lane == 0) set_status(c.workspace, wrong);
     return;
   }
-  constexpr int kVec = 16 / sizeof(T);
-  const int per = c.head_dim / kVec, all = c.kv_heads * per;
   T* const to = (T*)c.kv + p.a.layer * c.stride_layer + g * c.stride_page +
                 (int64_t)(t - q * c.page_size) * c.kv_heads * c.head_dim;
   T* const to_v = to + (int64_t)c.page_size * c.kv_heads * c.head_dim;
-  const T* const k = (const T*)p.a.k + b * p.a.k_stride_req + i * p.a.k_stride_pos;
-  const T* const v = (const T*)p.a.v + b * p.a.v_stride_req + i * p.a.v_stride_pos;
+#pragma unroll
+  for (int u = 0; u < kFirst; ++u)
+    if (lane + 32 * u < all) {
+      *(uint4*)(to + (int64_t)(lane + 32 * u) * kVec) = kx[u];
+      *(uint4*)(to_v + (int64_t)(lane + 32 * u) * kVec) = vx[u];
+    }
 #pragma unroll 4
-  for (int y = lane; y < all; y += 32) {
-    const int h = y / per, d = (y - h * per) * kVec;
-    const uint4 kx = *(const uint4*)(k + h * p.a.k_stride_head + d), vx = *(const uint4*)(v + h * p.a.v_stride_head + d);
-    *(uint4*)(to + (int64_t)y * kVec) = kx;
-    *(uint4*)(to_v + (int64_t)y * kVec) = vx;
+  for (int y = lane + 32 * kFirst; y < all; y += 32) {
+    const uint4 ky = row(k, p.a.k_stride_head, y), vy = row(v, p.a.v_stride_head, y);
+    *(uint4*)(to + (int64_t)y * kVec) = ky;
+    *(uint4*)(to_v + (int64_t)y * kVec) = vy;
   }
 }
 
