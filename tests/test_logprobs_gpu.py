@@ -98,3 +98,17 @@ def test_rows_past_32_bits_and_another_stream():
     assert float((got.logprob[:-1] + math.log(V)).abs().max()) < 1e-4
     assert float((got.entropy[:-1] - math.log(V)).abs().max()) < 1e-4
     assert int(got.top_ids[:-1].abs().max()) == 0
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [9, 31, 64, 200, 459, 767, 768, 1100])
+def test_short_rows_with_many_alternatives(dtype, V):
+    """Rows whose lanes hold a few tokens each, masks, ties and all."""
+    g = torch.Generator().manual_seed(V)
+    x = (2 * torch.randn(40, V, generator=g)).to(TYPES[dtype])
+    x[1::4][torch.rand(10, V, generator=g) < 0.5] = float("-inf")
+    x[2::4] = x[2::4].round()
+    x[3::8] = x[3::8].sort(1).values
+    x[:, V // 2] = 1.0
+    for top_n in (9, 17, 32):
+        check(x.cuda(), torch.randint(0, V, (40,), generator=g), top_n)

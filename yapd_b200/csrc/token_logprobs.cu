@@ -3,15 +3,15 @@
 // With m the largest logit, z = sum e^(x - m) and w = sum e^(x - m) (x - m):
 // log p(t) = x_t - m - ln z and the entropy is ln z - w / z, which has no
 // cancellation where one token has nearly all the mass. The alternatives need
-// no sort of the row: of the maxima of 32 disjoint parts of it, the n-th largest
+// no sort of the row: of the maxima of P disjoint parts of it, the n-th largest
 // has n tokens at or above it, so only tokens that reach it can be among the
-// first n. In a row without structure -32 ln(1 - n / 32) do, 9 for n = 8, 31 for
-// n = 20; they are listed and sorted.
+// first n. In a row without structure -P ln(1 - n / P) do, 9 for n = 8 and P = 32;
+// they are listed and ranked.
 //
 // A warp holds up to 1056 vectors of 16 bytes in its registers and makes all
 // passes over them alone; the parts are its lanes. A longer row, or few rows,
-// are shared out over the warps of a CTA or of a cluster; a part is then the
-// same lane of a CTA's warps, and the CTAs' tokens are merged at the end.
+// are shared out over the warps of a CTA or of a cluster; the parts are then the
+// lanes of a CTA, and the CTAs' tokens are merged at the end.
 #include <cooperative_groups.h>
 
 #include "select_common.cuh"
@@ -252,6 +252,24 @@ struct Tile {
         for (int k = g; k < g + kGroup; ++k) one(x[k]);
     if (rimmed) one(rim);
   }
+  // The lane's second largest logit (the largest one again if two are equal).
+  __device__ __forceinline__ float second() const {
+    float a = -INFINITY, b = -INFINITY;
+    const auto see = [&](const uint4& v) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 f = Pairs<T>::get(v, i);
+        b = fmaxf(b, fminf(a, f.x));
+        a = fmaxf(a, f.x);
+        b = fmaxf(b, fminf(a, f.y));
+        a = fmaxf(a, f.y);
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) see(x[k]);
+    if (rimmed) see(rim);
+    return b;
+  }
   // Calls f(vector, its number) for each vector with a token that reaches `reach`.
   template <class F>
   __device__ __forceinline__ void reaching(float reach, F f) const {
@@ -294,6 +312,18 @@ struct Candidates {
   int vectors, count;  // as many as reach the threshold, held or not
 };
 
+// The 32 largest of two lists, one ascending over the lanes and one descending: ascending.
+__device__ __forceinline__ float merge_top(float up, float down) {
+  const int lane = threadIdx.x & 31;
+  float x = fmaxf(up, down);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    const float y = __shfl_xor_sync(~0u, x, d);
+    x = lane & d ? fmaxf(x, y) : fminf(x, y);
+  }
+  return x;
+}
+
 // The n largest of `count` keys, in their order, to `top`: all different (but
 // for 0, none), each one's place is the number of those above it.
 template <int kSize>
@@ -309,7 +339,7 @@ __device__ __forceinline__ void place(const Key* keys, int count, int n, Key* to
 
 // The most likely tokens of vectors [v0, v1) of a row, by `kSize` threads that
 // `sync` brings together: to c.top. `tile(f)` calls f for the vectors that reach
-// `reach`, the n-th largest maximum of 32 parts.
+// `reach`, the n-th largest maximum of the parts.
 template <class T, int kSize, class Sync, class Tiles>
 __device__ __forceinline__ void find_top(const Row<T>& row, int v0, int v1, int n, float reach, Candidates& c, int rank,
                                          Sync sync, Tiles tiles) {
@@ -402,7 +432,20 @@ __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_const
     Key top = 0;
     if (kTop) {
       const int n = p.a.top_n;
-      const float reach = __shfl_sync(~0u, yapd::warp_bitonic_asc_f(mine), 32 - n);
+      const float firsts = yapd::warp_bitonic_asc_f(mine);
+      float reach = __shfl_sync(~0u, firsts, 32 - n);
+      if (n > (kVecs == kFew ? 8 : 20)) {
+        // The n-th largest of the lanes' 64 first and second logits lies closer to the
+        // n-th largest of all, where n comes near the number of lanes or the lanes
+        // have few tokens (7312 rows of 459, 32 alternatives: 23 us, and 105 us with
+        // the first ones alone, which every token reached). It is the largest, over
+        // all i, of the smaller of the i-th first and the (n - i)-th second one.
+        const float seconds = yapd::warp_bitonic_asc_f(tile.second());
+        const int rest = n - lane;  // lane i takes i first ones
+        const float f = __shfl_sync(~0u, firsts, (32 - lane) & 31), g = __shfl_sync(~0u, seconds, (32 - rest) & 31);
+        const float both = fminf(lane ? f : INFINITY, rest > 0 ? g : INFINITY);
+        reach = fmaxf(reach, warp_max(rest >= 0 ? both : -INFINITY));
+      }
       Candidates& c = candidates[warp];
       find_top<T, 32>(row, 0, row.vectors, n, reach, c, lane, [] { __syncwarp(); }, [&](auto f) { tile.reaching(reach, f); });
       top = c.top[lane];
@@ -453,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, kSomeFit) row_kernel(const __grid_co
   if (kOnce) tile.load(row, v0, v1);
   float mine = -INFINITY;
   tiles([&] { mine = fmaxf(mine, tile.largest()); });
-  if (kTop) mt.mine[tid] = mine;
+  if (kTop) mt.mine[tid] = yapd::warp_bitonic_asc_f(mine);
   const float m = warp_max(mine);
   unsigned long long z2 = 0, w2 = 0;
   tiles([&] { tile.add(m == -INFINITY ? 0.0f : m, z2, w2); });
@@ -461,10 +504,10 @@ __global__ void __launch_bounds__(kThreads, kSomeFit) row_kernel(const __grid_co
   if (lane == 0) mt.part[warp] = part;
   __syncthreads();
   if (kTop) {
-    float bucket = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) bucket = fmaxf(bucket, mt.mine[w * 32 + lane]);
-    const float reach = __shfl_sync(~0u, yapd::warp_bitonic_asc_f(bucket), 32 - n);
+    // the 32 largest of the lanes' maxima
+    static_assert(kWarps == 4, "two and two");
+    const float a0 = merge_top(mt.mine[lane], mt.mine[63 - lane]), a1 = merge_top(mt.mine[64 + lane], mt.mine[127 - lane]);
+    const float reach = __shfl_sync(~0u, merge_top(a0, __shfl_sync(~0u, a1, 31 - lane)), 32 - n);
     find_top<T, kThreads>(row, first(0), first(kWarps), n, reach, mt.c, tid, [] { __syncthreads(); },
                           [&](auto f) { tiles([&] { tile.reaching(reach, f); }); });
   }
