@@ -1,8 +1,9 @@
 // Log probabilities of given tokens, the entropy and the most likely tokens.
 //
-// With m the largest logit, z = sum e^(x - m) and w = sum e^(x - m) (x - m):
-// log p(t) = x_t - m - ln z and the entropy is ln z - w / z, which has no
-// cancellation where one token has nearly all the mass. The alternatives need
+// With m the largest logit, t = sum e^(x - m) over all tokens but one that has it,
+// and w = sum e^(x - m) (x - m): log p = x - m - ln(1 + t) and the entropy is
+// ln(1 + t) - w / (1 + t). Where one token has nearly all the mass, t is the
+// result: no sum of it has a 1 in it, whose last place would be the error. The alternatives need
 // no sort of the row: of the maxima of P disjoint parts of it, the n-th largest
 // has n tokens at or above it, so only tokens that reach it can be among the
 // first n. In a row without structure -P ln(1 - n / P) do, 9 for n = 8 and P = 32;
@@ -68,6 +69,8 @@ struct Pairs<float> {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
   __device__ static float largest(uint32_t a) { return __uint_as_float(a); }
+  // all ones in the halves of `a` that are above those of `b`
+  __device__ static uint32_t above(uint32_t a, uint32_t b) { return __uint_as_float(a) > __uint_as_float(b) ? ~0u : 0u; }
 };
 template <>
 struct Pairs<__nv_bfloat16> {
@@ -83,6 +86,9 @@ struct Pairs<__nv_bfloat16> {
   }
   __device__ static float largest(uint32_t a) {
     return fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u));
+  }
+  __device__ static uint32_t above(uint32_t a, uint32_t b) {
+    return __hgt2_mask(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
   }
 };
 template <>
@@ -101,6 +107,9 @@ struct Pairs<__half> {
     const float2 f = __half22float2(*reinterpret_cast<__half2*>(&a));
     return fmaxf(f.x, f.y);
   }
+  __device__ static uint32_t above(uint32_t a, uint32_t b) {
+    return __hgt2_mask(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -115,18 +124,26 @@ __device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsig
   return r;
 }
 
-// Sums over a part of a row against its own maximum: z = sum e^(x - m), w = sum e^(x - m) (x - m).
+// Sums over a part of a row against its own maximum: w = sum e^(x - m) (x - m),
+// tail = sum e^(x - m) without one token that has the maximum.
 struct Part {
-  float m, z, w;
+  float m, tail, w;
 };
 // `b` joins `a`: both against the larger maximum.
 __device__ __forceinline__ Part join(const Part& a, const Part& b) {
   const bool left = a.m >= b.m;
   const Part &big = left ? a : b, &small = left ? b : a;
-  if (small.m == -INFINITY) return Part{big.m, a.z + b.z, a.w + b.w};
-  const float d = fmaxf(small.m - big.m, -1e30f), f = expf(d);
-  return Part{big.m, fmaf(f, small.z, big.z), fmaf(f, fmaf(d, small.z, small.w), big.w)};
+  if (small.m == -INFINITY) return Part{big.m, a.tail + b.tail, a.w + b.w};  // nothing, or NaN
+  const float d = fmaxf(small.m - big.m, -1e30f), f = expf(d), z = 1.0f + small.tail;
+  return Part{big.m, fmaf(f, z, big.tail), fmaf(f, fmaf(d, z, small.w), big.w)};
 }
+
+// A lane's largest logit, and the first of the group of vectors that has it.
+constexpr int kRim = -1, kNowhere = -2;
+struct Most {
+  float value;
+  int group;
+};
 
 // A row's vectors: its first one begins at the 16-byte boundary at or below the
 // row, its last one ends at or after the row's end.
@@ -213,23 +230,36 @@ struct Tile {
   __device__ __forceinline__ static uint32_t word_of(const uint4& v) {
     return Pairs<T>::larger(Pairs<T>::larger(v.x, v.y), Pairs<T>::larger(v.z, v.w));
   }
-  // The lane's largest logit.
-  __device__ __forceinline__ float largest() {
-    uint32_t word = Pairs<T>::hidden();
+  // The lane's largest logit. In 16 bits a word holds two maxima, and `at` the group of each.
+  __device__ __forceinline__ Most largest() {
+    constexpr uint32_t kBoth = sizeof(T) == 2 ? 0x10001u : 1u, kRimAt = kVecs / kGroup;
+    uint32_t word = Pairs<T>::hidden(), at = 0;
+    const auto see = [&](uint32_t w, uint32_t g) {
+      const uint32_t more = Pairs<T>::above(w, word);
+      at = (at & ~more) | (g * kBoth & more);
+      word = Pairs<T>::larger(word, w);
+    };
 #pragma unroll
     for (int g = 0; g < kVecs; g += kGroup)
-      if (v0 + g * 32 < v1)
+      if (v0 + g * 32 < v1) {
+        uint32_t w = word_of(x[g]);
 #pragma unroll
-        for (int k = g; k < g + kGroup; ++k) word = Pairs<T>::larger(word, word_of(x[k]));
-    if (rimmed) word = Pairs<T>::larger(word, word_of(rim));
+        for (int k = g + 1; k < g + kGroup; ++k) w = Pairs<T>::larger(w, word_of(x[k]));
+        see(w, g / kGroup);
+      }
+    if (rimmed) see(word_of(rim), kRimAt);
     // 16-bit elements are converted anew: kept as 32-bit numbers they would not fit the registers.
     if constexpr (sizeof(T) == 2)
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) asm volatile("" : "+r"(x[k].x), "+r"(x[k].y), "+r"(x[k].z), "+r"(x[k].w));
-    return Pairs<T>::largest(word);
+    if constexpr (sizeof(T) == 2) {
+      const float2 f = Pairs<T>::get(make_uint4(word, 0, 0, 0), 0);
+      at = f.x >= f.y ? at & 0xffffu : at >> 16;
+    }
+    return Most{Pairs<T>::largest(word), at == kRimAt ? kRim : v0 + (int)at * kGroup * 32};
   }
-  // Adds the lane's sums against `base`: two each, for the even and the odd elements.
-  __device__ __forceinline__ void add(float base, unsigned long long& z2, unsigned long long& w2) const {
+  // Adds the lane's sums against `base`: two each, for the even and the odd elements. Group `skip` is left out of z2.
+  __device__ __forceinline__ void add(float base, int skip, unsigned long long& z2, unsigned long long& w2) const {
     const unsigned long long minus = yapd::f2_pack(-base, -base), log2e = yapd::f2_pack(yapd::kLog2e, yapd::kLog2e);
     const auto one = [&](const uint4& v) {
 #pragma unroll
@@ -247,10 +277,17 @@ struct Tile {
     };
 #pragma unroll
     for (int g = 0; g < kVecs; g += kGroup)
-      if (v0 + g * 32 < v1)
+      if (v0 + g * 32 < v1) {
+        const unsigned long long before = z2;
 #pragma unroll
         for (int k = g; k < g + kGroup; ++k) one(x[k]);
-    if (rimmed) one(rim);
+        if (v0 + g * 32 == skip) z2 = before;
+      }
+    if (rimmed) {
+      const unsigned long long before = z2;
+      one(rim);
+      if (skip == kRim) z2 = before;
+    }
   }
   // The lane's second largest logit (the largest one again if two are equal).
   __device__ __forceinline__ float second() const {
@@ -287,21 +324,55 @@ struct Tile {
   }
 };
 
-// The warp's sums from its lanes'.
-__device__ __forceinline__ Part warp_part(float m, unsigned long long z2, unsigned long long w2) {
-  Part p{m, 0.0f, 0.0f};
-  float y;
-  yapd::f2_unpack(z2, p.z, y);
-  p.z += y;
-  yapd::f2_unpack(w2, p.w, y);
-  p.w += y;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    p.z += __shfl_xor_sync(~0u, p.z, d);
-    p.w += __shfl_xor_sync(~0u, p.w, d);
+// The token of a warp's vectors that its tail leaves out: one lane that has the
+// maximum leaves its group out of its sum, and the warp adds the group's other
+// tokens, one to a lane (five more instructions to a group of vectors and a read that the
+// sums hide: 2 us of 52 for 8192 rows of 8194).
+template <class T>
+struct Apart {
+  static constexpr int kVec = Row<T>::kVec;
+  static_assert(kGroup * kVec <= 32, "a token to a lane");
+  float m;
+  int skip;     // the lane's group that is left out
+  float other;  // the lane's token of that group
+
+  // `most`: the lane's, of vectors [.., to) of the row.
+  __device__ __forceinline__ Apart(const Row<T>& row, const Most& most, int to) {
+    const int lane = threadIdx.x & 31;
+    m = warp_max(most.value);
+    const uint32_t have = __ballot_sync(~0u, most.value == m);
+    // nothing but -inf and NaN: none is left out
+    const int owner = m > -INFINITY ? __ffs(have) - 1 : -1, group = __shfl_sync(~0u, most.group, max(owner, 0));
+    skip = lane == owner ? group : kNowhere;
+    other = -INFINITY;
+    const int inner0 = row.lead ? 1 : 0, inner1 = (row.V + row.lead) / kVec, i = lane / kVec;
+    int j = group + i * 32 + owner, first = inner0, end = i < kGroup ? min(inner1, to) : 0;
+    if (group == kRim) {
+      j = owner == 0 ? 0 : inner1;
+      first = 0;
+      end = i == 0 ? row.vectors : 0;
+    }
+    const int id = j * kVec - row.lead + lane % kVec;
+    if (owner >= 0 && j >= first && j < end && id >= 0 && id < row.V) other = to_f32(row.x[id]);
   }
-  return p;
-}
+
+  // The warp's sums from its lanes'.
+  __device__ __forceinline__ Part join(unsigned long long z2, unsigned long long w2) const {
+    const int lane = threadIdx.x & 31, out = __ffs(__ballot_sync(~0u, other == m)) - 1;
+    Part p{m, lane == out || other == -INFINITY ? 0.0f : ex2((other - m) * yapd::kLog2e), 0.0f};
+    float x, y;
+    yapd::f2_unpack(z2, x, y);
+    p.tail += x + y;
+    yapd::f2_unpack(w2, p.w, y);
+    p.w += y;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+      p.tail += __shfl_xor_sync(~0u, p.tail, d);
+      p.w += __shfl_xor_sync(~0u, p.w, d);
+    }
+    return p;
+  }
+};
 
 // What the threads of a row put together for its alternatives: a warp's, or a CTA's.
 struct Candidates {
@@ -397,15 +468,15 @@ __device__ __forceinline__ void find_top(const Row<T>& row, int v0, int v1, int 
 template <class T>
 __device__ __forceinline__ void write(const yapd_logprobs_args& a, const Row<T>& row, int r, const Part& all, Key top) {
   const int lane = threadIdx.x & 31;
-  // NaN or +inf make z NaN; nothing but -inf leaves no maximum
-  const bool fine = all.m > -INFINITY && all.z > 0.0f && all.z < INFINITY;
-  const float lz = logf(all.z);
+  // NaN makes the tail NaN; nothing but -inf leaves no maximum
+  const bool fine = all.m > -INFINITY && all.m < INFINITY && all.tail < INFINITY;
+  const float lz = log1pf(all.tail);
   if (lane == 0) {
     if (a.targets) {
       const int64_t t = a.targets[r];
       a.logprob[r] = fine && t >= 0 && t < a.V ? to_f32(row.x[t]) - all.m - lz : NAN;
     }
-    if (a.entropy) a.entropy[r] = fine ? lz - all.w / all.z : NAN;
+    if (a.entropy) a.entropy[r] = fine ? lz - all.w / (1.0f + all.tail) : NAN;
   }
   if (lane < a.top_n) {
     a.top_ids[(int64_t)r * a.top_n + lane] = fine && top ? id_of(top) : -1;
@@ -426,9 +497,11 @@ __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_const
     const Row<T> row(p.a, (int)r);
     Tile<T, kVecs> tile;
     tile.load(row, 0, row.vectors);
-    const float mine = tile.largest(), m = warp_max(mine);
+    const Most most = tile.largest();
+    const Apart<T> apart(row, most, row.vectors);
+    const float mine = most.value, m = apart.m;
     unsigned long long z2 = 0, w2 = 0;
-    tile.add(m == -INFINITY ? 0.0f : m, z2, w2);
+    tile.add(m == -INFINITY ? 0.0f : m, apart.skip, z2, w2);
     Key top = 0;
     if (kTop) {
       const int n = p.a.top_n;
@@ -450,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_const
       find_top<T, 32>(row, 0, row.vectors, n, reach, c, lane, [] { __syncwarp(); }, [&](auto f) { tile.reaching(reach, f); });
       top = c.top[lane];
     }
-    write(p.a, row, (int)r, warp_part(m, z2, w2), top);
+    write(p.a, row, (int)r, apart.join(z2, w2), top);
     __syncwarp();
   }
 }
@@ -494,13 +567,17 @@ __global__ void __launch_bounds__(kThreads, kSomeFit) row_kernel(const __grid_co
     }
   };
   if (kOnce) tile.load(row, v0, v1);
-  float mine = -INFINITY;
-  tiles([&] { mine = fmaxf(mine, tile.largest()); });
-  if (kTop) mt.mine[tid] = yapd::warp_bitonic_asc_f(mine);
-  const float m = warp_max(mine);
+  Most most{-INFINITY, kNowhere};
+  tiles([&] {
+    const Most x = tile.largest();
+    if (x.value > most.value) most = x;
+  });
+  if (kTop) mt.mine[tid] = yapd::warp_bitonic_asc_f(most.value);
+  const Apart<T> apart(row, most, v1);
+  const float m = apart.m;
   unsigned long long z2 = 0, w2 = 0;
-  tiles([&] { tile.add(m == -INFINITY ? 0.0f : m, z2, w2); });
-  Part part = warp_part(m, z2, w2);
+  tiles([&] { tile.add(m == -INFINITY ? 0.0f : m, apart.skip, z2, w2); });
+  Part part = apart.join(z2, w2);
   if (lane == 0) mt.part[warp] = part;
   __syncthreads();
   if (kTop) {
