@@ -990,10 +990,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         ask();
       }
     }
-    copies_wait();  // what is on its way lands before the CTA ends
-    if (it < units)
-      for (int n = max(it - S::kStages, 0); n < it; ++n)
-        yapd::mbar_wait_bounded(&sh.full[n % S::kStages], n / S::kStages & 1, kWaitNs);
+    // What is on its way lands before the CTA ends and its shared memory is
+    // another one's, whichever side gave up: the last stages' copies are waited for
+    // here as well (they have landed where the other warps did not give up).
+    copies_wait();
+    for (int n = max(it - S::kStages, 0); n < it; ++n)
+      yapd::mbar_wait_bounded(&sh.full[n % S::kStages], n / S::kStages & 1, kWaitNs);
     if (it < units && lane == 0) {
       set_status(c.workspace, YAPD_STATUS_WAIT_TIMEOUT);
       atomicExch(&sh.given_up, 1);
