@@ -161,6 +161,11 @@ __device__ __forceinline__ void copy_group(uint32_t to, const CUtensorMap* map, 
       "l"(map), "r"(smem_addr(bar)), "r"(0), "r"(token), "r"(head), "r"(page)
       : "memory");
 }
+// A warp's bounded wait: its lanes go on or give up together, since every lane
+// has a clock of its own and the products and shuffles that follow need them all.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int64_t limit_ns) {
+  return __all_sync(~0u, yapd::mbar_wait_bounded(bar, parity, limit_ns));
+}
 // Arrives at `bar` when all earlier copies of this thread have landed.
 __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -898,7 +903,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     int it = 0;
     for (int stage = 0, phase = 1; it < units; ++it) {
       // a stage's first use needs no wait: the phase before the first counts as over
-      if (!yapd::mbar_wait_bounded(&sh.empty[stage], phase, it < S::kStages ? kWaitNs : p.wait_ns)) break;
+      if (!warp_wait(&sh.empty[stage], phase, it < S::kStages ? kWaitNs : p.wait_ns)) break;
       const int k0 = tile_start(at, shift);
       const uint32_t to = smem_addr(ring + stage * S::kStage);
       uint32_t tokens[kPer];
@@ -995,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     // here as well (they have landed where the other warps did not give up).
     copies_wait();
     for (int n = max(it - S::kStages, 0); n < it; ++n)
-      yapd::mbar_wait_bounded(&sh.full[n % S::kStages], n / S::kStages & 1, kWaitNs);
+      warp_wait(&sh.full[n % S::kStages], n / S::kStages & 1, kWaitNs);
     if (it < units && lane == 0) {
       set_status(c.workspace, YAPD_STATUS_WAIT_TIMEOUT);
       atomicExch(&sh.given_up, 1);
@@ -1026,12 +1031,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     auto meet = [&]() {
       __syncwarp();
       if (lane == 0) yapd::mbar_arrive(&sh.met);
-      ok = ok && yapd::mbar_wait_bounded(&sh.met, meetings++ & 1, p.wait_ns);
+      ok = ok && warp_wait(&sh.met, meetings++ & 1, p.wait_ns);
     };
     Rows<T, D, M> w;
     bool fresh = true, whole = true;
     for (int it = 0, stage = 0, phase = 0; it < units; ++it) {
-      if (!(ok = yapd::mbar_wait_bounded(&sh.full[stage], phase, p.wait_ns))) break;
+      if (!(ok = warp_wait(&sh.full[stage], phase, p.wait_ns))) break;
       const Tile& t = sh.tile[stage];
       const int head0 = t.head0, rb = t.rb;
       if (fresh) {
