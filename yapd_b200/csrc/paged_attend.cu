@@ -233,6 +233,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// What is carried as a row's maximum is kUp below it, so that a weight is up to
+// 2^kUp: in half precision the smallest number is 2^-24, and weights below 2^-25 of
+// the largest one, which thousands of tokens may have, would leave the sums of the
+// values while z counts them. From 2^14 down the halves of a weight reach 2^-38 of
+// the largest. The other types have the exponents of 32 bits.
+template <class T>
+constexpr float kUp = 0.0f;
+template <>
+constexpr float kUp<__half> = 14.0f;
+
 // ------------------------------------------------------------------ the rows
 
 // One thread's share of a warp's M query rows (g = lane / 4, t = lane % 4).
@@ -569,7 +579,7 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Pl
     for (int n = 0; n < N / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    const float m = fmaxf(w.m[r], top * p.scale_log2);  // the scale is not negative (see `negate`)
+    const float m = fmaxf(w.m[r], fmaf(top, p.scale_log2, -kUp<T>));  // the scale is not negative (see `negate`)
     base[r] = m == -INFINITY ? 0.0f : m;
     fix[r] = ex2(w.m[r] - base[r]);
     moved |= fix[r] != 1.0f;
@@ -740,11 +750,12 @@ __device__ __forceinline__ void write_row(const Attend& p, int b, int head, int 
     *(uint2*)out = x;
   }
 }
+template <class T>
 __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int row, float m, float z) {
   if (!p.a.lse) return;
   const int i = (int)div_floor(row, p.groups), h = head * p.group + row - i * p.group;
   p.a.lse[((int64_t)b * p.a.new_tokens + i) * p.a.heads + h] =
-      z == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(z);
+      z == 0.0f ? -INFINITY : (m + kUp<T>) * 0.69314718055994531f + logf(z * exp2f(-kUp<T>));
 }
 
 // The kernel. Its bound is the rate of the pages' reads: a token's key and value
@@ -1015,7 +1026,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         const int r = x / (D / 4), h = r % p.a.heads, i = r / p.a.heads, head = h / p.group;
         const int row = i * p.group + h - head * p.group;
         write_row<T>(p, b, head, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
-        if (x % (D / 4) == 0) write_lse(p, b, head, row, 0.0f, 0.0f);
+        if (x % (D / 4) == 0) write_lse<T>(p, b, head, row, 0.0f, 0.0f);
       }
     }
     const int wk_all = kWarps / p.wr, wk = warp / p.wr, wrow = warp - wk * p.wr;
@@ -1104,7 +1115,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
           if (whole) {
             const float rz = z == 0.0f ? 0.0f : 1.0f / z;
             write_row<T>(p, b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
-            if (d == 0) write_lse(p, b, head0 + hi, rb * block_rows + row, m, z);
+            if (d == 0) write_lse<T>(p, b, head0 + hi, rb * block_rows + row, m, z);
           } else {
             *(float4*)(left_at + 4 * x) = o;
             if (d == 0) *(float2*)(left_at + kMaxRows * D + 2 * rr) = make_float2(m, z);
@@ -1195,7 +1206,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here;
     const int full = piece.rb * block_rows + rr - hi * rows_here;
     write_row<T>(p, piece.b, piece.head0 + hi, full, 4 * d, o, z == 0.0f ? 0.0f : 1.0f / z);
-    if (d == 0) write_lse(p, piece.b, piece.head0 + hi, full, m, z);
+    if (d == 0) write_lse<T>(p, piece.b, piece.head0 + hi, full, m, z);
   }
 }
 
