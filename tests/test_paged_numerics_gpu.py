@@ -29,3 +29,18 @@ def test_small_weights_under_large_ones(dtype, heads, kv_heads, T, window, sinks
             kv[0, table[s][j // 16], 1, j % 16] = 0.0
     out, lse = cache.attend(0, q.cuda(), window=window, sinks=sinks, return_lse=True)
     check(cache, q, out, lse, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.125, -1.5, 1e-44, 2.0])
+@pytest.mark.parametrize("heads,kv_heads,T,causal,window,sinks", [(4, 4, 1, True, 0, 0), (8, 2, 5, True, 0, 0), (8, 4, 2, False, 0, 0),
+                                                                  (8, 1, 3, True, 30, 7), (4, 2, 16, False, 20, 3)])
+def test_scales(dtype, scale, heads, kv_heads, T, causal, window, sinks):
+    """A scale of 0 gives the mean of what is seen; a negative one turns the order of the scores."""
+    cache, q, k, v = make((16, 29, 64, 333), dtype=TYPES[dtype], heads=heads, kv_heads=kv_heads, T=T, layers=1)
+    mask = dict(causal=causal, window=window, sinks=sinks)
+    out, lse = cache.attend(0, q.cuda(), scale=scale, return_lse=True, **mask)
+    if scale < 0:       # the bounds go by the products' sizes: the same attention of the negative queries
+        check(cache, -q, out, lse, scale=-scale, **mask)
+    else:
+        check(cache, q, out, lse, scale=scale, **mask)

@@ -46,8 +46,9 @@ struct Attend {
   int hg;            // key heads of a unit: 1, 2, 4
   int head_groups, row_blocks;
   bool boxes;        // pages are whole groups of 16 tokens
+  uint32_t keep;     // bits of the queries that count: none where the scale is 0
   uint32_t negate;   // sign bits of the queries to turn
-  float scale_log2;  // not negative
+  float scale_log2;  // positive
   int64_t wait_ns;   // limit of each wait
   Piece* pieces;     // (gridDim): the cut piece that begins in the CTA's share
   float* partials;   // (gridDim, 2) of (kMaxRows, D) sums and (kMaxRows, 2) maxima and sums of weights
@@ -306,7 +307,7 @@ __device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D, M>& w, co
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           w.q[k][r + R::kOwn * e] =
-              row < p.rows ? *(const uint32_t*)(q + 16 * k + 8 * e + 2 * t) ^ p.negate : 0u;
+              row < p.rows ? (*(const uint32_t*)(q + 16 * k + 8 * e + 2 * t) & p.keep) ^ p.negate : 0u;
     }
   } else {
     __syncwarp();
@@ -314,6 +315,7 @@ __device__ __forceinline__ void begin_rows(const Attend& p, Rows<T, D, M>& w, co
       const int r = x / (D / 4), d = x % (D / 4) * 4, row = row0 + r;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (row < p.rows) v = *(const float4*)(query_at<T>(p, c.b, head, row) + d);
+      if (!p.keep) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (p.negate) v = make_float4(-v.x, -v.y, -v.z, -v.w);
       *(float4*)(qs + r * (D + 4) + d) = v;
     }
@@ -579,7 +581,7 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Pl
     for (int n = 0; n < N / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    const float m = fmaxf(w.m[r], fmaf(top, p.scale_log2, -kUp<T>));  // the scale is not negative (see `negate`)
+    const float m = fmaxf(w.m[r], fmaf(top, p.scale_log2, -kUp<T>));  // the scale is positive (see `keep`, `negate`)
     base[r] = m == -INFINITY ? 0.0f : m;
     fix[r] = ex2(w.m[r] - base[r]);
     moved |= fix[r] != 1.0f;
@@ -1370,9 +1372,11 @@ extern "C" int yapd_attend(const yapd_attend_args* args, void* stream) {
   p.group = a.heads / kvh;
   p.groups = make_div((uint32_t)p.group);
   p.rows = a.new_tokens * p.group;
-  // a negative scale is a positive one of the negative queries
+  // A negative scale is a positive one of the negative queries, and a scale of 0
+  // any other one of queries that are 0: hidden scores are -inf before the scale.
+  p.keep = a.scale == 0.0f ? 0u : ~0u;
   p.negate = std::signbit(a.scale) ? dt == YAPD_DTYPE_F32 ? 0x80000000u : 0x80008000u : 0u;
-  p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
+  p.scale_log2 = a.scale == 0.0f ? 1.0f : std::fabs(a.scale) * 1.4426950408889634f;
   p.wait_ns = a.wait_limit_ns ? a.wait_limit_ns : kWaitNs;
   char* const scratch = (char*)a.cache.workspace + kHeaderBytes + pages_scratch_bytes(a.cache);
   p.pieces = (Piece*)scratch;
