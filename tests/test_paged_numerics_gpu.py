@@ -44,3 +44,58 @@ def test_scales(dtype, scale, heads, kv_heads, T, causal, window, sinks):
         check(cache, -q, out, lse, scale=-scale, **mask)
     else:
         check(cache, q, out, lse, scale=scale, **mask)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,T,causal,window,sinks", [(4, 4, 1, True, 0, 0), (8, 2, 1, True, 0, 0), (8, 4, 3, True, 0, 0),
+                                                                  (8, 1, 1, False, 0, 0), (8, 2, 16, False, 0, 0), (6, 3, 2, True, 90, 5)])
+@pytest.mark.parametrize("j,score", [(0, 0), (2, 30), (40, 3), (77, -10), (100, 40), (150, -22), (199, 0), (199, 25), (160, -60)])
+def test_infinite_values_that_are_seen(dtype, heads, kv_heads, T, causal, window, sinks, j, score):
+    """A value that is infinite makes the output infinite wherever its tile lies, for the rows that see it and
+    whatever its weight; values of both signs and NaN make it NaN; the other dims do not change."""
+    n = 200
+    cache, q, k, v = make((n, 33), dtype=TYPES[dtype], heads=heads, kv_heads=kv_heads, T=T, layers=1, fill=0.0, seed=j)
+    kv, row = cache.kv, cache.page_table[0].tolist()
+    q[..., 0] = 8.0
+    kv[0, :, 0, :, :, 0] = 0.0
+    kv[0, row[j // 16], 0, j % 16, :, 0] = score          # 64^-0.5 * 8 = 1
+    mask = dict(causal=causal, window=window, sinks=sinks)
+    want, want_l = cache.attend(0, q.cuda(), return_lse=True, **mask)
+    inf = float("inf")
+    kv[0, row[j // 16], 1, j % 16, :, 3] = inf
+    kv[0, row[j // 16], 1, j % 16, :, 17] = -inf
+    kv[0, row[j // 16], 1, j % 16, :, 40] = float("nan")
+    kv[0, row[j // 16], 1, j % 16, :, 63] = inf
+    kv[0, row[n // 2 // 16], 1, n // 2 % 16, :, 63] = -inf if j != n // 2 else float("nan")
+    out, lse = cache.attend(0, q.cuda(), return_lse=True, **mask)
+    assert torch.equal(lse, want_l)
+    for i in range(T):
+        p = n - T + i
+        sees = lambda t: (not causal or t <= p) and (not window or t > p - window or t < sinks)  # noqa: E731
+        if sees(j):
+            assert bool((out[0, i, :, 3] == inf).all()) and bool((out[0, i, :, 17] == -inf).all())
+            assert bool(out[0, i, :, 40].isnan().all())
+        if sees(j) and sees(n // 2):
+            assert bool(out[0, i, :, 63].isnan().all())
+        rest = [d for d in range(64) if d not in ((3, 17, 40, 63) if sees(j) else (63,) if sees(n // 2) else ())]
+        assert torch.equal(out[0, i][:, rest], want[0, i][:, rest])
+    assert torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("ps,T", [(16, 1), (100, 1), (7, 12), (64, 32)])
+def test_infinite_values_of_long_requests(dtype, ps, T):
+    """The same where a request is cut and joined; NaN scores stay NaN."""
+    n, inf = 9000, float("inf")
+    cache, q, k, v = make((n, 700), dtype=TYPES[dtype], heads=8, kv_heads=4, T=T, layers=1, ps=ps, fill=0.0)
+    kv, table = cache.kv, cache.page_table.tolist()
+    for j, d in ((0, 1), (1234, 2), (4321, 3), (8800, 4)):
+        kv[0, table[0][j // ps], 1, j % ps, 2, d] = inf if d % 2 else -inf
+    out, lse = cache.attend(0, q.cuda(), causal=False, return_lse=True)
+    assert bool((out[0, :, 4:6, 1:4:2] == inf).all()) and bool((out[0, :, 4:6, 2:5:2] == -inf).all())
+    assert int((~torch.isfinite(out)).sum()) == T * 2 * 4
+    kv[0, table[0][5000 // ps], 0, 5000 % ps, 2, 0] = float("nan")
+    nan, lse_nan = cache.attend(0, q.cuda(), causal=False, return_lse=True)
+    assert bool(nan[0, :, 4:6].isnan().all()) and bool(lse_nan[0, :, 4:6].isnan().all())
+    rest = [h for h in range(8) if h not in (4, 5)]
+    assert torch.equal(nan[:, :, rest], out[:, :, rest]) and torch.equal(nan[1], out[1])

@@ -641,6 +641,81 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Pl
   values<T, D, M, N, false>(w.o, s, at);
 }
 
+// The keys that a warp has added to its sums.
+struct Added {
+  int b, len, shift;      // request, its tokens, tiles of 2^shift
+  int tile0, tile1;       // of these tiles ...
+  int first, span;        // ... `span` keys from `first` on
+};
+
+// The sum of the values of dim `dim` that are not finite, of the keys that a row
+// with the bounds `end` and `low` sees: infinite, NaN, or 0 where all are finite.
+template <class T>
+__device__ __noinline__ float not_finite(const Attend& p, Added a, int head, int dim, int end, int low) {
+  const yapd_cache& c = p.a.cache;
+  const Span span = span_of(p, a.len, a.shift);
+  const int slot = p.a.slots ? p.a.slots[a.b] : a.b, sinks = sinks_of(p);
+  const int32_t* const row = c.page_table + (int64_t)slot * c.max_pages;
+  const T* const vals = (const T*)c.kv + p.a.layer * c.stride_layer +
+                        ((int64_t)c.page_size * c.kv_heads + head) * c.head_dim + dim;
+  float odd = 0.0f;
+  for (int tile = a.tile0; tile <= a.tile1; ++tile) {
+    const int j0 = ((tile < span.sink_tiles ? tile : tile + span.skip) << a.shift) + a.first, j1 = min(j0 + a.span, end);
+#pragma unroll 4
+    for (int j = j0; j < j1; ++j) {
+      if (j < low && j >= sinks) continue;
+      const int q = (int)div_floor(j, p.page), g = row[q];
+      if (g < 0 || g >= c.pages) continue;
+      const float f = to_f32(vals[g * c.stride_page + (int64_t)(j - q * c.page_size) * c.kv_heads * c.head_dim]);
+      if (!isfinite(f)) odd += f;
+    }
+    if (isnan(odd)) break;
+  }
+  return odd;
+}
+
+// The largest size of three numbers, NaN if one is.
+__device__ __forceinline__ float larger_size(float x, float y, float z) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+  return m;
+}
+
+// An infinite value makes a sum infinite, but its products with the two halves of a
+// weight may be NaN: the second half may be 0 or negative. Where a sum is not
+// finite, the values that made it so are read once more. Once to a piece: the steps
+// would have to wait for their products to look at them (128 rows of 16 positions:
+// 113 us instead of 107).
+template <class T, int D, int M>
+__device__ __forceinline__ void make_good(const Attend& p, Rows<T, D, M>& w, const Added& a, int head) {
+  using R = Rows<T, D, M>;
+  if constexpr (sizeof(T) == 2) {
+    float most = 0.0f;
+#pragma unroll
+    for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+      for (int e = 0; e < R::kEach; e += 2) most = larger_size(most, w.o[d][e], w.o[d][e + 1]);
+    if (!__any_sync(~0u, !(most < INFINITY))) return;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    int end[2], low[2];  // of the rows that the thread's sums are of
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int from = R::kTurned ? ((2 * t + r) & (M - 1)) * 4 : lane, own = R::kTurned ? 0 : r;
+      end[r] = __shfl_sync(~0u, w.end[own], from);
+      low[r] = __shfl_sync(~0u, w.low[own], from);
+    }
+#pragma unroll
+    for (int d = 0; d < R::kSums; ++d)
+#pragma unroll
+      for (int k = 0; k < R::kEach; ++k)
+        if (!isfinite(w.o[d][k])) {
+          const int r = R::kTurned ? k & 1 : k >> 1, dim = R::kTurned ? 16 * d + g + 8 * (k >> 1) : 8 * d + 2 * t + (k & 1);
+          const float odd = not_finite<T>(p, a, head, dim, end[r], low[r]);
+          if (odd != 0.0f) w.o[d][k] = odd;  // 0: finite values whose sum is not
+        }
+  }
+}
+
 // Where the sums of a row's dim `d` meet: rows that are stored together lie in different banks.
 template <int D>
 __device__ __forceinline__ int meet_at(int row, int d) { return row * D + (d ^ ((row ^ row >> 2) & 3) << 3); }
@@ -1048,12 +1123,14 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     };
     Rows<T, D, M> w;
     bool fresh = true, whole = true;
+    int tile0 = 0;  // the piece's first one here
     for (int it = 0, stage = 0, phase = 0; it < units; ++it) {
       if (!(ok = warp_wait(&sh.full[stage], phase, p.wait_ns))) break;
       const Tile& t = sh.tile[stage];
       const int head0 = t.head0, rb = t.rb;
       if (fresh) {
         whole = t.tile == 0;
+        tile0 = t.tile;
         Cursor x;
         x.b = t.b;
         x.len = t.len;
@@ -1088,6 +1165,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         whole = whole && done;
         const int b = t.b;
         const long long start = u0 + it - t.tile, end = start + t.tiles;
+        make_good<T, D, M>(p, w, Added{b, t.len, shift, tile0, t.tile, part * span, span}, head0 + head_in);
         meet();
         if (!ok) break;
         float* const joined = (float*)(ring + stage * S::kStage);
