@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(Pages p) {
     } else {
       const int64_t add = tokens_of(p, i);
       len = len_of(p, s);
-      if (add < 0 || len + add > (int64_t)c.max_pages * p.page.d) {
+      if (add < 0 || add > (int64_t)c.max_pages * p.page.d - len) {
         set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
       } else {
         first = (int)div_floor(len + p.page.d - 1, p.page);
