@@ -34,8 +34,11 @@ extern "C" {
                                          hold too was not made */
 #define YAPD_STATUS_BAD_SLOT 128u     /* a slot out of range, listed twice, or a
                                          fork's target that is not empty */
-#define YAPD_STATUS_BAD_LENGTH 256u   /* more tokens than the slot's table holds,
-                                         or fewer than the call names */
+#define YAPD_STATUS_BAD_LENGTH 256u   /* a length or a reserve of more tokens than
+                                         the slot's table holds, a negative one,
+                                         a truncate of more tokens than there are,
+                                         a store of more than there are (those
+                                         before the slot's first are not made) */
 
 /* New tokens per request of one attention call. */
 #define YAPD_MAX_NEW_TOKENS 32
@@ -53,6 +56,9 @@ extern "C" {
  * blocks, so a pool may be layer-major or page-major.  Token t of slot s is
  * token t % page_size of page page_table[s][t / page_size]; a table entry of
  * -1 is no page (a request that was trimmed has them in its middle).
+ * A slot with a length that is negative or more than its table holds is read
+ * as an empty one and left as it is (YAPD_STATUS_BAD_LENGTH), but for a truncate
+ * with tokens < 0, which empties it.
  * refs[p] is the number of table entries that hold page p; 0: free.  There is
  * no list of free pages: the lowest-numbered free page is always the next one
  * given out, so that a sequence of calls always gives the same tables.

@@ -91,6 +91,7 @@ struct Shape {
 
 // ----------------------------------------------------------------- the cache
 
+// Tokens of a request; none where its length does not fit its table.
 __device__ __forceinline__ int slot_len(const Attend& p, int b, int& slot) {
   const yapd_cache& c = p.a.cache;
   slot = p.a.slots ? p.a.slots[b] : b;
@@ -98,8 +99,8 @@ __device__ __forceinline__ int slot_len(const Attend& p, int b, int& slot) {
     slot = -1;
     return 0;
   }
-  const int64_t n = c.kv_len[slot], most = (int64_t)c.max_pages * c.page_size;
-  return (int)(n < 0 ? 0 : n > most ? most : n);
+  const int64_t n = c.kv_len[slot];
+  return fits(c, n) ? (int)n : 0;
 }
 
 // What the queries of a request of `len` tokens see: tokens below `sinks`, and
@@ -895,7 +896,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
     int slot;
     const int len = slot_len(p, b, slot);
     mine += (long long)span_of(p, len, shift).tiles * pairs;
-    if (slot < 0 && blockIdx.x == 0) set_status(c.workspace, YAPD_STATUS_BAD_SLOT);
+    if (blockIdx.x == 0) {
+      if (slot < 0)
+        set_status(c.workspace, YAPD_STATUS_BAD_SLOT);
+      else if (!fits(c, c.kv_len[slot]))
+        set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
+    }
   }
   long long upto = mine;
 #pragma unroll

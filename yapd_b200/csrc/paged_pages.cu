@@ -69,10 +69,10 @@ __device__ __forceinline__ int slot_of(const Pages& p, int i) {
   return s >= 0 && s < p.c.slots ? s : -1;
 }
 
-// Tokens of a slot, within what its table holds.
+// Tokens of a slot, or -1 where that does not fit its table.
 __device__ __forceinline__ int len_of(const Pages& p, int slot) {
-  const int64_t n = p.c.kv_len[slot], most = (int64_t)p.c.max_pages * p.page.d;
-  return (int)(n < 0 ? 0 : n > most ? most : n);
+  const int64_t n = p.c.kv_len[slot];
+  return fits(p.c, n) ? (int)n : -1;
 }
 
 __device__ __forceinline__ int64_t tokens_of(const Pages& p, int i) {
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kMetaThreads) reserve_kernel(Pages p) {
     } else {
       const int64_t add = tokens_of(p, i);
       len = len_of(p, s);
-      if (add < 0 || add > (int64_t)c.max_pages * p.page.d - len) {
+      if (len < 0 || add < 0 || add > (int64_t)c.max_pages * p.page.d - len) {
         set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
       } else {
         first = (int)div_floor(len + p.page.d - 1, p.page);
@@ -228,7 +228,12 @@ __global__ void __launch_bounds__(128) fork_kernel(Pages p) {
     return;
   }
   __syncthreads();
-  const int len = len_of(p, from), held = (int)div_floor(len + p.page.d - 1, p.page);
+  const int len = len_of(p, from);
+  if (len < 0) {
+    if (threadIdx.x == 0) set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
+    return;
+  }
+  const int held = (int)div_floor(len + p.page.d - 1, p.page);
   const int32_t* in = c.page_table + (int64_t)from * c.max_pages;
   int32_t* out = c.page_table + (int64_t)s * c.max_pages;
   for (int j = threadIdx.x; j < held; j += blockDim.x) {
@@ -255,7 +260,14 @@ __global__ void __launch_bounds__(128) release_kernel(Pages p, bool trim) {
     if (threadIdx.x == 0) set_status(c.workspace, YAPD_STATUS_BAD_SLOT);
     return;
   }
-  const int len = len_of(p, s), held = (int)div_floor(len + p.page.d - 1, p.page);
+  const int64_t take = trim ? 0 : tokens_of(p, i);
+  int len = len_of(p, s);
+  if (len < 0) {
+    if (threadIdx.x == 0) set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
+    if (take >= 0) return;
+    len = c.max_pages * p.page.d;  // freed: whatever the table holds goes
+  }
+  const int held = (int)div_floor(len + p.page.d - 1, p.page);
   int32_t* row = c.page_table + (int64_t)s * c.max_pages;
   if (trim) {
     // the next token stands at `len` and sees j > len - window, or j < sinks
@@ -264,7 +276,6 @@ __global__ void __launch_bounds__(128) release_kernel(Pages p, bool trim) {
       if ((int64_t)j * p.page.d >= p.sinks && (int64_t)(j + 1) * p.page.d <= reach) give_up(c, row + j);
     return;
   }
-  const int64_t take = tokens_of(p, i);
   if (take > len && threadIdx.x == 0) set_status(c.workspace, YAPD_STATUS_BAD_LENGTH);
   const int keep = take < 0 || take > len ? 0 : len - (int)take;
   __syncthreads();  // every thread has read the length

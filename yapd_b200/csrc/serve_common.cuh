@@ -84,6 +84,11 @@ inline int check_cache(const yapd_cache& c) {
   return YAPD_OK;
 }
 
+// Whether a slot's length is one that its table can hold.
+__device__ __forceinline__ bool fits(const yapd_cache& c, int64_t n) {
+  return n >= 0 && n <= (int64_t)c.max_pages * c.page_size;
+}
+
 __device__ __forceinline__ void set_status(void* workspace, uint32_t bits) {
   atomicOr(static_cast<uint32_t*>(workspace), bits);
 }
