@@ -95,7 +95,8 @@ size_t yapd_cache_workspace_size(const yapd_cache* cache);
  * every score is -inf.  Products and sums are in 32 bits.
  *
  * k and v, where given, are the new tokens' rows: the call stores them in the
- * request's pages and attends over them.  Rows are q + b*q_stride_req +
+ * request's pages and attends over them (of the requests that name the same slot
+ * only the first one's are stored: YAPD_STATUS_BAD_SLOT).  Rows are q + b*q_stride_req +
  * i*q_stride_pos + h*q_stride_head (elements; likewise k, v, out), head_dim
  * contiguous elements, 16-byte aligned.  The types are the cache's.
  */

@@ -780,9 +780,15 @@ __global__ void __launch_bounds__(128) store_kernel(const __grid_constant__ Atte
     }
   int slot;
   const int t = slot_len(p, b, slot) - p.a.new_tokens + i;
+  // of the requests that name a slot the first one stores
+  bool again = false;
+  if (p.a.slots)
+#pragma unroll 4
+    for (int j = lane; j < b; j += 32) again |= p.a.slots[j] == slot;
+  again = __any_sync(~0u, again);
   uint32_t wrong = 0;
   int g = -1, q = 0;
-  if (slot < 0) {
+  if (slot < 0 || again) {
     wrong = YAPD_STATUS_BAD_SLOT;
   } else if (t < 0) {
     wrong = YAPD_STATUS_BAD_LENGTH;
