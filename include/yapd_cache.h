@@ -73,7 +73,8 @@ typedef struct yapd_cache {
   int64_t* kv_len;              /* (slots,) tokens of each slot */
   int32_t* refs;                /* (pages,) */
   void* workspace;              /* zero-filled before its first use; its calls
-                                   are ordered on one stream */
+                                   are ordered on one stream, each one's
+                                   launches together: one thread at a time */
   size_t workspace_bytes;
 } yapd_cache;
 

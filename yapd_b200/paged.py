@@ -25,6 +25,7 @@ twice) leaves the slot alone and sets bits of ``cache.status()``.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -42,7 +43,8 @@ class PagedCache:
     updated in place; ``PagedCache.empty`` makes them.  Each page's block has to
     be contiguous; the first two strides of ``kv`` are free.  ``head_dim`` is 32,
     64, 96 or 128.  The cache's calls share a workspace: they are ordered on one
-    stream, or by events where a program uses several.
+    stream, or by events where a program uses several.  Threads may share a
+    cache: a call's arguments and launches are one step to the others.
     """
 
     def __init__(self, kv: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, refs: torch.Tensor):
@@ -82,6 +84,8 @@ class PagedCache:
             raise ValueError("page_size, kv_heads or max_pages * page_size is out of range")
         self._workspace = torch.zeros(need, dtype=torch.uint8, device=dev)
         c.workspace, c.workspace_bytes = self._workspace.data_ptr(), need
+        # the argument structures are kept from call to call, and a call's kernels share the workspace
+        self._lock = threading.Lock()
         self._pages = N.PagesArgs()
         self._cache = self._pages.cache = c
         self._scale, self._plans = self._dim ** -0.5, {}
@@ -141,11 +145,8 @@ class PagedCache:
             raise ValueError("sinks must not be negative")
         if slots is not None:
             self._check_list("slots", slots, B)
-            a.slots = slots.data_ptr()
         elif B > self.slots:
             raise ValueError(f"{B} requests, but {self.slots} slots")
-        else:
-            a.slots = None
         at = q.data_ptr()
         if copies or at % 16 or (k is not None and (k.data_ptr() % 16 or v.data_ptr() % 16)):
             # rows that the kernels cannot read: contiguous copies
@@ -154,9 +155,6 @@ class PagedCache:
                 k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
             return self.attend(layer, q, k, v, slots=slots, causal=causal, window=window, sinks=sinks, scale=scale,
                                out=out, return_lse=return_lse, wait_limit_ns=wait_limit_ns)
-        a.q = at
-        if k is not None:
-            a.k, a.v = k.data_ptr(), v.data_ptr()
         if out is None:
             out = torch.empty_like(out_like)
         else:
@@ -164,13 +162,18 @@ class PagedCache:
             if out.shape != shape or out.dtype != self._dtype or out.get_device() != self._index or \
                     out.data_ptr() % 16 or self._unreadable(o):
                 raise ValueError(f"out must be a {tuple(shape)} {self._dtype} tensor on {self.device} whose rows are aligned")
-        a.out = out.data_ptr()
-        a.out_stride_req, a.out_stride_pos, a.out_stride_head = (o[0], 0, o[1]) if len(o) == 3 else o[:3]
         lse = torch.empty_like(lse_like) if return_lse else None
-        a.lse = lse.data_ptr() if return_lse else None
-        a.layer, a.scale = layer, self._scale if scale is None else scale
-        a.causal, a.window, a.sinks, a.wait_limit_ns = 1 if causal else 0, window, sinks, wait_limit_ns
-        self._call(self._lib.yapd_attend, a)
+        with self._lock:
+            a.q = at
+            if k is not None:
+                a.k, a.v = k.data_ptr(), v.data_ptr()
+            a.slots = None if slots is None else slots.data_ptr()
+            a.out = out.data_ptr()
+            a.out_stride_req, a.out_stride_pos, a.out_stride_head = (o[0], 0, o[1]) if len(o) == 3 else o[:3]
+            a.lse = lse.data_ptr() if return_lse else None
+            a.layer, a.scale = layer, self._scale if scale is None else scale
+            a.causal, a.window, a.sinks, a.wait_limit_ns = 1 if causal else 0, window, sinks, wait_limit_ns
+            self._call(self._lib.yapd_attend, a)
         return (out, lse) if return_lse else out
 
     def _unreadable(self, strides) -> bool:
@@ -222,63 +225,56 @@ class PagedCache:
         slot that the pool has no room for, and all after it, are refused."""
         if isinstance(tokens, int) and tokens < 0:
             raise ValueError("tokens must not be negative")
-        p = self._listed(slots)
-        self._tokens(tokens, p.n)
-        granted = torch.empty(p.n, dtype=torch.bool, device=self.device)
-        p.granted = granted.data_ptr()
-        self._call(self._lib.yapd_pages_reserve, p)
+        n, at = self._listed(slots)
+        same, each = self._tokens(tokens, n)
+        granted = torch.empty(n, dtype=torch.bool, device=self.device)
+        self._change(self._lib.yapd_pages_reserve, n=n, slots=at, tokens=same, tokens_each=each,
+                     granted=granted.data_ptr())
         return granted
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """The empty slots ``dst`` become copies of ``src`` and share their pages
         (both int32 ``(n,)``; no slot is in both)."""
-        p = self._listed(dst)
-        self._check_list("src", src, p.n)
-        p.src = src.data_ptr()
-        self._call(self._lib.yapd_pages_fork, p)
+        n, at = self._listed(dst)
+        self._check_list("src", src, n)
+        self._change(self._lib.yapd_pages_fork, n=n, slots=at, src=src.data_ptr())
 
     def truncate(self, tokens, slots: torch.Tensor | None = None) -> None:
         """Takes the last ``tokens`` (an int, or int64 ``(n,)``) from each slot."""
         if isinstance(tokens, int) and tokens < 0:
             raise ValueError("tokens must not be negative")
-        p = self._listed(slots)
-        self._tokens(tokens, p.n)
-        self._call(self._lib.yapd_pages_truncate, p)
+        n, at = self._listed(slots)
+        same, each = self._tokens(tokens, n)
+        self._change(self._lib.yapd_pages_truncate, n=n, slots=at, tokens=same, tokens_each=each)
 
     def free(self, slots: torch.Tensor | None = None) -> None:
         """Empties the slots; pages that no other slot holds become free."""
-        p = self._listed(slots)
-        p.tokens, p.tokens_each = -1, None
-        self._call(self._lib.yapd_pages_truncate, p)
+        n, at = self._listed(slots)
+        self._change(self._lib.yapd_pages_truncate, n=n, slots=at, tokens=-1, tokens_each=None)
 
     def trim(self, window: int, sinks: int = 0, slots: torch.Tensor | None = None) -> None:
         """Gives up the pages that attention with this ``window`` and ``sinks``
         no longer sees, from the slots' next token on."""
         if window < 1 or sinks < 0:
             raise ValueError("window must be positive and sinks not negative")
-        p = self._listed(slots)
-        p.window, p.sinks = window, sinks
-        self._call(self._lib.yapd_pages_trim, p)
+        n, at = self._listed(slots)
+        self._change(self._lib.yapd_pages_trim, n=n, slots=at, window=window, sinks=sinks)
 
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the pool's lowest numbers, in all layers and
         tables.  Returns their number, a ``(1,)`` int32 device tensor."""
-        p = self._listed(None)
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        p.live = live.data_ptr()
-        self._call(self._lib.yapd_pages_compact, p)
+        self._change(self._lib.yapd_pages_compact, n=0, live=live.data_ptr())
         return live
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Copies pages ``src`` to ``dst`` (int32 ``(n,)``) in all layers; no page
         is both read and written, or written twice."""
-        p = self._pages
         if dst.dim() != 1 or dst.shape[0] > self.kv.shape[1]:
             raise ValueError("dst must be (n,) with n at most the number of pages")
         self._check_list("dst", dst, dst.shape[0])
         self._check_list("src", src, dst.shape[0])
-        p.n, p.src, p.dst = dst.shape[0], src.data_ptr(), dst.data_ptr()
-        self._call(self._lib.yapd_pages_copy, p)
+        self._change(self._lib.yapd_pages_copy, n=dst.shape[0], src=src.data_ptr(), dst=dst.data_ptr())
 
     # ---------------------------------------------------------------- status
 
@@ -305,28 +301,31 @@ class PagedCache:
         if rc:
             N.check(rc)
 
+    def _change(self, entry, **fields) -> None:
+        with self._lock:
+            for name, value in fields.items():
+                setattr(self._pages, name, value)
+            self._call(entry, self._pages)
+
     def _check_list(self, name: str, t: torch.Tensor, n: int) -> None:
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != self._index or \
                 (n > 1 and t.stride(0) != 1):
             raise ValueError(f"{name} must be a contiguous int32 ({n},) tensor on {self.device}")
 
     def _listed(self, slots: torch.Tensor | None):
-        p = self._pages
+        """Length and address of a list of slots (none: all of them)."""
         if slots is None:
-            p.n, p.slots = self.slots, None
-        else:
-            if slots.dim() != 1 or slots.shape[0] > self.slots:
-                raise ValueError(f"slots must be (n,) with n <= {self.slots}")
-            self._check_list("slots", slots, slots.shape[0])
-            p.n, p.slots = slots.shape[0], slots.data_ptr()
-        return p
+            return self.slots, None
+        if slots.dim() != 1 or slots.shape[0] > self.slots:
+            raise ValueError(f"slots must be (n,) with n <= {self.slots}")
+        self._check_list("slots", slots, slots.shape[0])
+        return slots.shape[0], slots.data_ptr()
 
-    def _tokens(self, tokens, n: int) -> None:
-        p = self._pages
+    def _tokens(self, tokens, n: int):
+        """A number for all of the list, or the address of one for each."""
         if isinstance(tokens, torch.Tensor):
             if tokens.dtype != torch.int64 or tuple(tokens.shape) != (n,) or tokens.device != self.device or \
                     not tokens.is_contiguous():
                 raise ValueError(f"tokens must be an int or a contiguous int64 ({n},) tensor on {self.device}")
-            p.tokens, p.tokens_each = 0, tokens.data_ptr()
-        else:
-            p.tokens, p.tokens_each = int(tokens), None
+            return 0, tokens.data_ptr()
+        return int(tokens), None
