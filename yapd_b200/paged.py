@@ -228,8 +228,10 @@ class PagedCache:
         n, at = self._listed(slots)
         same, each = self._tokens(tokens, n)
         granted = torch.empty(n, dtype=torch.bool, device=self.device)
-        self._change(self._lib.yapd_pages_reserve, n=n, slots=at, tokens=same, tokens_each=each,
-                     granted=granted.data_ptr())
+        p = self._pages
+        with self._lock:
+            p.n, p.slots, p.tokens, p.tokens_each, p.granted = n, at, same, each, granted.data_ptr()
+            self._call(self._lib.yapd_pages_reserve, p)
         return granted
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -237,20 +239,21 @@ class PagedCache:
         (both int32 ``(n,)``; no slot is in both)."""
         n, at = self._listed(dst)
         self._check_list("src", src, n)
-        self._change(self._lib.yapd_pages_fork, n=n, slots=at, src=src.data_ptr())
+        p = self._pages
+        with self._lock:
+            p.n, p.slots, p.src = n, at, src.data_ptr()
+            self._call(self._lib.yapd_pages_fork, p)
 
     def truncate(self, tokens, slots: torch.Tensor | None = None) -> None:
         """Takes the last ``tokens`` (an int, or int64 ``(n,)``) from each slot."""
         if isinstance(tokens, int) and tokens < 0:
             raise ValueError("tokens must not be negative")
         n, at = self._listed(slots)
-        same, each = self._tokens(tokens, n)
-        self._change(self._lib.yapd_pages_truncate, n=n, slots=at, tokens=same, tokens_each=each)
+        self._truncate(n, at, *self._tokens(tokens, n))
 
     def free(self, slots: torch.Tensor | None = None) -> None:
         """Empties the slots; pages that no other slot holds become free."""
-        n, at = self._listed(slots)
-        self._change(self._lib.yapd_pages_truncate, n=n, slots=at, tokens=-1, tokens_each=None)
+        self._truncate(*self._listed(slots), -1, None)
 
     def trim(self, window: int, sinks: int = 0, slots: torch.Tensor | None = None) -> None:
         """Gives up the pages that attention with this ``window`` and ``sinks``
@@ -258,13 +261,19 @@ class PagedCache:
         if window < 1 or sinks < 0:
             raise ValueError("window must be positive and sinks not negative")
         n, at = self._listed(slots)
-        self._change(self._lib.yapd_pages_trim, n=n, slots=at, window=window, sinks=sinks)
+        p = self._pages
+        with self._lock:
+            p.n, p.slots, p.window, p.sinks = n, at, window, sinks
+            self._call(self._lib.yapd_pages_trim, p)
 
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the pool's lowest numbers, in all layers and
         tables.  Returns their number, a ``(1,)`` int32 device tensor."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
-        self._change(self._lib.yapd_pages_compact, n=0, live=live.data_ptr())
+        p = self._pages
+        with self._lock:
+            p.n, p.live = 0, live.data_ptr()
+            self._call(self._lib.yapd_pages_compact, p)
         return live
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -274,7 +283,10 @@ class PagedCache:
             raise ValueError("dst must be (n,) with n at most the number of pages")
         self._check_list("dst", dst, dst.shape[0])
         self._check_list("src", src, dst.shape[0])
-        self._change(self._lib.yapd_pages_copy, n=dst.shape[0], src=src.data_ptr(), dst=dst.data_ptr())
+        p = self._pages
+        with self._lock:
+            p.n, p.src, p.dst = dst.shape[0], src.data_ptr(), dst.data_ptr()
+            self._call(self._lib.yapd_pages_copy, p)
 
     # ---------------------------------------------------------------- status
 
@@ -301,11 +313,11 @@ class PagedCache:
         if rc:
             N.check(rc)
 
-    def _change(self, entry, **fields) -> None:
+    def _truncate(self, n, at, same, each) -> None:
+        p = self._pages
         with self._lock:
-            for name, value in fields.items():
-                setattr(self._pages, name, value)
-            self._call(entry, self._pages)
+            p.n, p.slots, p.tokens, p.tokens_each = n, at, same, each
+            self._call(self._lib.yapd_pages_truncate, p)
 
     def _check_list(self, name: str, t: torch.Tensor, n: int) -> None:
         if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != self._index or \
