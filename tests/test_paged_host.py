@@ -4,6 +4,7 @@ import re
 import threading
 import time
 
+import numpy as np
 import pytest
 import torch
 
@@ -88,3 +89,20 @@ def test_threads_do_not_share_a_call(cache):
         if name == "yapd_pages_truncate":
             p = N.PagesArgs.from_buffer_copy(b)
             assert (p.n, p.tokens, p.tokens_each is None) in ((2, 0, False), (3, -1, True))
+
+
+def test_numbers_that_do_not_fit_are_refused(cache):
+    """Nothing is cut off to 64 bits on its way to the library: 2^64 - 1 tokens are not -1, which empties a slot."""
+    q = torch.zeros(2, 4, 32)
+    for call in (lambda: cache.truncate(2 ** 64 - 1), lambda: cache.truncate(2 ** 64 + 1), lambda: cache.truncate(np.int64(-1)),
+                 lambda: cache.reserve(2 ** 63), lambda: cache.reserve(np.int32(-5)), lambda: cache.trim(2 ** 64 + 3),
+                 lambda: cache.trim(3, 2 ** 64), lambda: cache.attend(0, q, window=2 ** 63),
+                 lambda: cache.attend(0, q, sinks=2 ** 64 + 1)):
+        with pytest.raises(ValueError):
+            call()
+    assert cache._lib.calls == []
+    cache.truncate(np.int64(3))
+    cache.trim(2 ** 63 - 1, 2 ** 63 - 1)
+    cache.attend(0, q, window=2 ** 63 - 1)
+    cache.attend(0, q, window=-1)
+    assert len(cache._lib.calls) == 4

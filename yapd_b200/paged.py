@@ -33,6 +33,8 @@ from . import _native as N
 
 _DTYPES = {torch.float32: N.YAPD_DTYPE_F32, torch.bfloat16: N.YAPD_DTYPE_BF16, torch.float16: N.YAPD_DTYPE_F16}
 
+_MOST = 2 ** 63 - 1  # larger numbers would be cut off on their way to the library
+
 
 class PagedCache:
     """Pages ``kv`` ``(layers, pages, 2, page_size, kv_heads, head_dim)`` in
@@ -141,8 +143,8 @@ class PagedCache:
             raise TypeError(f"q, k and v must be on {self.device}")
         if not 0 <= layer < self._layers:
             raise ValueError(f"layer {layer} of {self._layers}")
-        if sinks < 0:
-            raise ValueError("sinks must not be negative")
+        if not 0 <= sinks <= _MOST or window > _MOST:
+            raise ValueError("sinks must not be negative, and sinks and window fit 64 bits")
         if slots is not None:
             self._check_list("slots", slots, B)
         elif B > self.slots:
@@ -223,8 +225,6 @@ class PagedCache:
         the list, in its order; ``kv_len`` grows.  A partly filled last page that
         other slots hold too is copied first.  Returns ``(n,)`` bool: the first
         slot that the pool has no room for, and all after it, are refused."""
-        if isinstance(tokens, int) and tokens < 0:
-            raise ValueError("tokens must not be negative")
         n, at = self._listed(slots)
         same, each = self._tokens(tokens, n)
         granted = torch.empty(n, dtype=torch.bool, device=self.device)
@@ -246,8 +246,6 @@ class PagedCache:
 
     def truncate(self, tokens, slots: torch.Tensor | None = None) -> None:
         """Takes the last ``tokens`` (an int, or int64 ``(n,)``) from each slot."""
-        if isinstance(tokens, int) and tokens < 0:
-            raise ValueError("tokens must not be negative")
         n, at = self._listed(slots)
         self._truncate(n, at, *self._tokens(tokens, n))
 
@@ -258,8 +256,8 @@ class PagedCache:
     def trim(self, window: int, sinks: int = 0, slots: torch.Tensor | None = None) -> None:
         """Gives up the pages that attention with this ``window`` and ``sinks``
         no longer sees, from the slots' next token on."""
-        if window < 1 or sinks < 0:
-            raise ValueError("window must be positive and sinks not negative")
+        if not 1 <= window <= _MOST or not 0 <= sinks <= _MOST:
+            raise ValueError("window must be positive and sinks not negative, and both fit 64 bits")
         n, at = self._listed(slots)
         p = self._pages
         with self._lock:
@@ -340,4 +338,7 @@ class PagedCache:
                     not tokens.is_contiguous():
                 raise ValueError(f"tokens must be an int or a contiguous int64 ({n},) tensor on {self.device}")
             return 0, tokens.data_ptr()
-        return int(tokens), None
+        tokens = int(tokens)
+        if not 0 <= tokens <= _MOST:
+            raise ValueError(f"tokens must not be negative, and fit 64 bits, got {tokens}")
+        return tokens, None
