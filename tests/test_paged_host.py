@@ -97,7 +97,7 @@ def test_numbers_that_do_not_fit_are_refused(cache):
     for call in (lambda: cache.truncate(2 ** 64 - 1), lambda: cache.truncate(2 ** 64 + 1), lambda: cache.truncate(np.int64(-1)),
                  lambda: cache.reserve(2 ** 63), lambda: cache.reserve(np.int32(-5)), lambda: cache.trim(2 ** 64 + 3),
                  lambda: cache.trim(3, 2 ** 64), lambda: cache.attend(0, q, window=2 ** 63),
-                 lambda: cache.attend(0, q, sinks=2 ** 64 + 1)):
+                 lambda: cache.attend(0, q, window=5 - 2 ** 64), lambda: cache.attend(0, q, sinks=2 ** 64 + 1)):
         with pytest.raises(ValueError):
             call()
     assert cache._lib.calls == []

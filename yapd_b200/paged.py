@@ -143,7 +143,7 @@ class PagedCache:
             raise TypeError(f"q, k and v must be on {self.device}")
         if not 0 <= layer < self._layers:
             raise ValueError(f"layer {layer} of {self._layers}")
-        if not 0 <= sinks <= _MOST or window > _MOST:
+        if not 0 <= sinks <= _MOST or not -_MOST <= window <= _MOST:
             raise ValueError("sinks must not be negative, and sinks and window fit 64 bits")
         if slots is not None:
             self._check_list("slots", slots, B)
