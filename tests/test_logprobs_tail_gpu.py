@@ -82,3 +82,11 @@ def test_ties_and_lone_tokens(dtype):
         for have, sign in ((got.logprob, 1), (got.top_logprobs[:, 0], 1), (got.entropy, -1)):
             err = (have.cpu().double() - sign * want).abs()
             assert bool((err <= (V / 64 + 64) * 2.0 ** -24 * want.abs()).all()), (V, err)
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    """2^32 + 3 rows are not 3."""
+    from yapd_b200.logprobs import token_logprobs
+    x = torch.zeros(1, 1, device="cuda").expand(2 ** 32 + 3, 1)
+    with pytest.raises(ValueError):
+        token_logprobs(x)

@@ -44,6 +44,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     if not 0 <= top_n <= N.YAPD_LOGPROBS_MAX_TOP:
         raise ValueError(f"top_n must be 0 to {N.YAPD_LOGPROBS_MAX_TOP}, got {top_n}")
     R, V = logits.shape
+    if R >= 2 ** 31:        # the kernels count rows in 32 bits
+        raise ValueError(f"logits must have fewer than 2^31 rows, got {R}")
     if (V > 1 and logits.stride(1) != 1) or (R > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
     dev, index = logits.device, logits.get_device()
