@@ -53,8 +53,8 @@ extern "C" {
  * then values, the page layout of the reference's FlashInfer engine
  * (chatterbox_flash/engines/flashinfer.py:110-115).  A block is contiguous;
  * stride_layer and stride_page (elements, multiples of 16 bytes) place the
- * blocks, so a pool may be layer-major or page-major.  Token t of slot s is
- * token t % page_size of page page_table[s][t / page_size]; a table entry of
+ * blocks, so a pool may be layer-major or page-major.  The keys of a page are at
+ * most 2^34 bytes.  Token t of slot s is token t % page_size of page page_table[s][t / page_size]; a table entry of
  * -1 is no page (a request that was trimmed has them in its middle).
  * A slot with a length that is negative or more than its table holds is read
  * as an empty one and left as it is (YAPD_STATUS_BAD_LENGTH), but for a truncate

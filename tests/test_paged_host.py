@@ -106,3 +106,17 @@ def test_numbers_that_do_not_fit_are_refused(cache):
     cache.attend(0, q, window=2 ** 63 - 1)
     cache.attend(0, q, window=-1)
     assert len(cache._lib.calls) == 4
+
+
+def test_pages_that_a_copy_could_not_count_are_refused():
+    """Half a page of 2^31 vectors of 16 bytes was copied as none."""
+    import ctypes as C
+
+    from tests.test_serve_abi import good_cache
+    from yapd_b200 import _native as N
+    c = good_cache(N)
+    c.head_dim, c.kv_heads, c.max_pages = 128, 1024, 2
+    for size, dtype, fits in ((32768, N.YAPD_DTYPE_F32, True), (32769, N.YAPD_DTYPE_F32, False),
+                              (65536, N.YAPD_DTYPE_F32, False), (65536, N.YAPD_DTYPE_BF16, True)):
+        c.page_size, c.dtype = size, dtype
+        assert (N.lib().yapd_cache_workspace_size(C.byref(c)) > 0) is fits

@@ -64,6 +64,8 @@ inline int check_cache_shape(const yapd_cache& c) {
     return YAPD_ERR_BAD_SHAPE;
   if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 96 && c.head_dim != 128) return YAPD_ERR_BAD_SHAPE;
   if (c.kv_heads > 1024 || c.page_size > 65536) return YAPD_ERR_BAD_SHAPE;
+  // the copies count the 16-byte vectors of half a page in 31 bits
+  if ((int64_t)c.page_size * c.kv_heads * c.head_dim * dtype_size(c.dtype) > (int64_t)1 << 34) return YAPD_ERR_BAD_SHAPE;
   // positions, rounded up to pages and tiles, stay below 2^31
   if ((int64_t)c.max_pages * c.page_size >= ((int64_t)1 << 31) - (1 << 17)) return YAPD_ERR_BAD_SHAPE;
   if (c.dtype != YAPD_DTYPE_F32 && c.dtype != YAPD_DTYPE_BF16 && c.dtype != YAPD_DTYPE_F16)
