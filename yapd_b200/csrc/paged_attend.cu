@@ -221,9 +221,21 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
   return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 __device__ __forceinline__ float2 unpack2(uint32_t x, __half) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
-// x and y as the sums of two T each
+// What a weight is multiplied with where it enters a product, and a sum of values
+// by the inverse of at its end. The smallest number in half precision is 2^-24:
+// weights below 2^-25 of the largest one, which thousands of tokens may have, would
+// leave the sums of the values while the sum of weights counts them. From 2^14 down
+// their halves reach 2^-38. The other types have the exponents of 32 bits.
+template <class T>
+constexpr float kUp = 1.0f;
+template <>
+constexpr float kUp<__half> = 16384.0f;
+
+// x and y, times kUp, as the sums of two T each
 template <class T>
 __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t& low) {
+  x *= kUp<T>;
+  y *= kUp<T>;
   high = pack2<T>(x, y);
   const float2 h = unpack2(high, T());
   low = pack2<T>(x - h.x, y - h.y);
@@ -234,16 +246,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// What is carried as a row's maximum is kUp below it, so that a weight is up to
-// 2^kUp: in half precision the smallest number is 2^-24, and weights below 2^-25 of
-// the largest one, which thousands of tokens may have, would leave the sums of the
-// values while z counts them. From 2^14 down the halves of a weight reach 2^-38 of
-// the largest. The other types have the exponents of 32 bits.
-template <class T>
-constexpr float kUp = 0.0f;
-template <>
-constexpr float kUp<__half> = 14.0f;
 
 // ------------------------------------------------------------------ the rows
 
@@ -582,7 +584,7 @@ __device__ __forceinline__ void step(const Attend& p, Rows<T, D, M>& w, const Pl
     for (int n = 0; n < N / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * r], s[n][2 * r + 1]));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    const float m = fmaxf(w.m[r], fmaf(top, p.scale_log2, -kUp<T>));  // the scale is positive (see `keep`, `negate`)
+    const float m = fmaxf(w.m[r], top * p.scale_log2);  // the scale is positive (see `keep`, `negate`)
     base[r] = m == -INFINITY ? 0.0f : m;
     fix[r] = ex2(w.m[r] - base[r]);
     moved |= fix[r] != 1.0f;
@@ -834,12 +836,11 @@ __device__ __forceinline__ void write_row(const Attend& p, int b, int head, int 
     *(uint2*)out = x;
   }
 }
-template <class T>
 __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int row, float m, float z) {
   if (!p.a.lse) return;
   const int i = (int)div_floor(row, p.groups), h = head * p.group + row - i * p.group;
   p.a.lse[((int64_t)b * p.a.new_tokens + i) * p.a.heads + h] =
-      z == 0.0f ? -INFINITY : (m + kUp<T>) * 0.69314718055994531f + logf(z * exp2f(-kUp<T>));
+      z == 0.0f ? -INFINITY : m * 0.69314718055994531f + logf(z);
 }
 
 // The kernel. Its bound is the rate of the pages' reads: a token's key and value
@@ -1115,7 +1116,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
         const int r = x / (D / 4), h = r % p.a.heads, i = r / p.a.heads, head = h / p.group;
         const int row = i * p.group + h - head * p.group;
         write_row<T>(p, b, head, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 1.0f);
-        if (x % (D / 4) == 0) write_lse<T>(p, b, head, row, 0.0f, 0.0f);
+        if (x % (D / 4) == 0) write_lse(p, b, head, row, 0.0f, 0.0f);
       }
     }
     const int wk_all = kWarps / p.wr, wk = warp / p.wr, wrow = warp - wk * p.wr;
@@ -1205,9 +1206,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, M>::kFit) attend_kernel(
             o.w = fmaf(f, v.w, o.w);
           }
           if (whole) {
-            const float rz = z == 0.0f ? 0.0f : 1.0f / z;
+            const float rz = z == 0.0f ? 0.0f : 1.0f / (kUp<T> * z);
             write_row<T>(p, b, head0 + hi, rb * block_rows + row, 4 * d, o, rz);
-            if (d == 0) write_lse<T>(p, b, head0 + hi, rb * block_rows + row, m, z);
+            if (d == 0) write_lse(p, b, head0 + hi, rb * block_rows + row, m, z);
           } else {
             *(float4*)(left_at + 4 * x) = o;
             if (d == 0) *(float2*)(left_at + kMaxRows * D + 2 * rr) = make_float2(m, z);
@@ -1297,8 +1298,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     }
     const int rr = x / (D / 4), d = x - rr * (D / 4), hi = rr / rows_here;
     const int full = piece.rb * block_rows + rr - hi * rows_here;
-    write_row<T>(p, piece.b, piece.head0 + hi, full, 4 * d, o, z == 0.0f ? 0.0f : 1.0f / z);
-    if (d == 0) write_lse<T>(p, piece.b, piece.head0 + hi, full, m, z);
+    write_row<T>(p, piece.b, piece.head0 + hi, full, 4 * d, o, z == 0.0f ? 0.0f : 1.0f / (kUp<T> * z));
+    if (d == 0) write_lse(p, piece.b, piece.head0 + hi, full, m, z);
   }
 }
 
