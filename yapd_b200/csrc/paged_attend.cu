@@ -846,16 +846,16 @@ __device__ __forceinline__ void write_lse(const Attend& p, int b, int head, int 
 // The kernel. Its bound is the rate of the pages' reads: a token's key and value
 // row, 4 D bytes at 16 bits, meet 4 D rows operations, so up to about 100 query
 // rows of a key head the products are the smaller part; they run on the
-// mma.sync pipe, whose tiles of 16 rows fit these counts (a tcgen05 tile has 64
-// or 128), at a tenth of its rate. What it took to get there, 256 requests of
+// mma.sync pipe, at a tenth of its rate for one row (from 16 rows on a tcgen05
+// tile with the keys or the queries on its 128 rows would shorten the steps). What it took to get there, 256 requests of
 // 16 heads of 64 and 20 to 1250 tokens (692 MB; 106 us at the copy rate):
 //   every warp copying its share of a stage, 255 registers       217 us
 //   products by the number of rows, four CTAs per SM             169 us
 //   one fetching warp, a 512-byte bulk copy to a token           161 us (17 ns a copy and SM)
 //   one fetching warp, 16 bytes a lane                           184 us
 //   one fetching warp, boxes of 16 tokens                        125 us
-// and 4 requests of 95k tokens with 8 key heads of 128 (1.63 GB) 250 us, 99.9 %
-// of the copy rate. One request of 417 tokens, a tile to a CTA, takes 10 us: 3.3
+// and 4 requests of 95k tokens with 8 key heads of 128 (1.63 GB) 247 to 255 us, the
+// copy rate. One request of 417 tokens, a tile to a CTA, takes 10 us: 3.3
 // us to the first box, 1 us for the tile, 2 us for what the warps and the joining
 // kernel add up, the rest for the three launches.
 

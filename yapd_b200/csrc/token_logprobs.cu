@@ -485,10 +485,10 @@ __device__ __forceinline__ void write(const yapd_logprobs_args& a, const Row<T>&
 }
 
 // Rows of one tile: a warp to each, nothing to wait for. 8192 rows of 8194 16-bit
-// logits (134 MB; 21 us at the copy rate) take 35 us, with eight alternatives 51
-// us: 2400 and 3200 instructions a row at half of the issue slots, since a row in
-// registers leaves room for twelve warps to an SM. Four warps to such a row: 36
-// and 53 us; a block of 256 threads: 49 and 77 us.
+// logits (134 MB; 21 us at the copy rate) take 37 us, with eight alternatives 52
+// us: 2500 and 3300 instructions a row at half of the issue slots, since a row in
+// registers leaves room for twelve warps to an SM. Four warps to such a row: 53
+// and 79 us.
 template <class T, bool kTop, int kVecs>
 __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_constant__ Logprobs p) {
   __shared__ Candidates candidates[kTop ? kWarps : 1];
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, kFit) rows_kernel(const __grid_const
       if (n > (kVecs == kFew ? 8 : 20)) {
         // The n-th largest of the lanes' 64 first and second logits lies closer to the
         // n-th largest of all, where n comes near the number of lanes or the lanes
-        // have few tokens (7312 rows of 459, 32 alternatives: 23 us, and 105 us with
+        // have few tokens (7312 rows of 459, 32 alternatives: 24 us, and 105 us with
         // the first ones alone, which every token reached). It is the largest, over
         // all i, of the smaller of the i-th first and the (n - i)-th second one.
         const float seconds = yapd::warp_bitonic_asc_f(tile.second());
@@ -539,10 +539,10 @@ struct Meeting {
 };
 
 // A CTA or a cluster to each row, a warp to each share of its vectors. kOnce: a
-// tile holds the share. 4096 rows of 8192 32-bit logits (134 MB) take 29 us, 71 % of
-// the copy rate; 384 rows of 128256 16-bit ones,
-// read twice, take 52 us (15 us at the copy rate), of which the alternatives are
-// 14; one row of 6563 takes 6 us, two meetings of the cluster's CTAs and launch.
+// tile holds the share. 4096 rows of 8192 32-bit logits (134 MB) take 31 us, 66 % of
+// the copy rate; 384 rows of 128256 16-bit ones, read twice and a third time for
+// the alternatives, take 38 us without them and 52 us with them (15 us at the copy
+// rate); one row of 6563 takes 6 us, two meetings of the cluster's CTAs and launch.
 template <class T, bool kTop, int kVecs, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kSomeFit) row_kernel(const __grid_constant__ Logprobs p) {
   __shared__ Meeting mt;
@@ -633,9 +633,9 @@ int launch(Logprobs& p, cudaStream_t st) {
   // One warp where it holds the row and there are rows for half of the warps,
   // or the row is short; else a CTA, and a cluster for so few rows that they
   // leave half of the GPU idle, as long as every lane has four vectors. (With
-  // 384 rows of 128256: clusters of four that hold the rows take 66 us, single
-  // CTAs that read them a second time out of L2 52 us; 4096 rows of 8192 in 32
-  // bits: 29 us with 18 vectors to a lane, 37 with 33, 33 with 9.)
+  // 384 rows of 128256: clusters of four that hold the rows take 58 us, single
+  // CTAs that read them again out of L2 52 us; 4096 rows of 8192 in 32 bits: 31 us
+  // with 18 vectors to a lane, 39 with 33, 37 with 9.)
   constexpr int kTile = kVecs * 32;
   if (vectors <= kTile && (a.R >= kSlots / 2 || vectors <= 64)) {
     const int ctas = (a.R + kWarps - 1) / kWarps, most = 148 * kFit;
