@@ -30,3 +30,21 @@ def test_the_first_request_of_a_slot_stores(dtype, B, T):
     cache.clear_status()
     again = cache.attend(0, qs.cuda(), slots=slots.cuda())      # reading a slot twice is fine
     assert cache.status() == 0 and torch.equal(again, out)
+
+
+def test_lists_that_begin_anywhere():
+    """The list of slots needs no alignment; a slot is found wherever it was named before."""
+    lens = [9, 40, 17, 33, 20]
+    for start in range(4):
+        for at in range(1, 9):
+            cache, q, k, v = make(lens, T=1, layers=1)
+            names = torch.zeros(start + 9, dtype=torch.int32)
+            names[start:] = torch.tensor([0, 1, 2, 3, 9, 9, 9, 9, 9])        # 9: no slot
+            names[start + at] = 4
+            names[start + 8] = 4
+            rows = torch.randn(9, 4, 64).to(torch.bfloat16)
+            cache.attend(0, rows.cuda(), rows.cuda(), rows.cuda(), slots=names.cuda()[start:])
+            first = at if at < 8 else 8
+            page = int(cache.page_table[4, 19 // 16])
+            assert torch.equal(cache.kv[0, page, 0, 19 % 16].cpu(), rows[first])
+            assert cache.status() == N.YAPD_STATUS_BAD_SLOT
