@@ -30,7 +30,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, *,
     any row stride), the rows' entropies, and the ``top_n <= 32`` most likely
     tokens of each row.
 
-    Arithmetic is in 32 bits.  A target outside ``[0, V)`` (the select step's -1)
+    Arithmetic is in 32 bits; the sum over the tokens leaves out the most likely
+    one, so that its log probability keeps its digits near 0.  A target outside ``[0, V)`` (the select step's -1)
     gives NaN.  Masked tokens (-inf) have probability 0 and are no alternatives;
     a row with fewer than ``top_n`` others ends in ids -1 with -inf.  A row with
     NaN or +inf, or with nothing but -inf, gives NaN and ids -1.

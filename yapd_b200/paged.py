@@ -42,7 +42,9 @@ class PagedCache:
 
     ``page_table`` ``(slots, max_pages)`` int32 (-1: no page), ``kv_len``
     ``(slots,)`` int64 and ``refs`` ``(pages,)`` int32 are the caller's tensors,
-    updated in place; ``PagedCache.empty`` makes them.  Each page's block has to
+    updated in place; ``PagedCache.empty`` makes them.  A slot whose length is
+    negative or more than its table holds is empty to ``attend`` and left alone by
+    the page operations, but for ``free``.  Each page's block has to
     be contiguous; the first two strides of ``kv`` are free.  ``head_dim`` is 32,
     64, 96 or 128.  The cache's calls share a workspace: they are ordered on one
     stream, or by events where a program uses several.  Threads may share a
@@ -116,7 +118,8 @@ class PagedCache:
         heads, D)`` for its last ``T <= 32``, with ``heads`` a multiple of
         ``kv_heads``; row ``b`` is slot ``slots[b]`` (int32), or slot ``b``.
         ``k`` and ``v`` (``q``'s shape with ``kv_heads``) are stored in the
-        tokens' pages by the same call; without them the pages are only read.
+        tokens' pages by the same call (of rows with the same slot the first one's);
+        without them the pages are only read.
         The tokens are part of ``kv_len`` already (``reserve``).  ``out``, if given,
         overlaps none of the inputs.
 
